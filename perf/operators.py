@@ -292,6 +292,7 @@ def _plain_logprobs(s):
     if s["case"]["K"]:
         # equal logits in the order of their indices
         value, index = torch.sort(x, dim=1, descending=True, stable=True)
+        index = torch.where(value == float("-inf"), -1, index)   # forbidden: no alternative
         s["top_ids"].copy_(index[:, : s["case"]["K"]])
         s["top_logprobs"].copy_(value[:, : s["case"]["K"]] - norm)
     return s["logprobs"], s["entropy"], s["top_ids"], s["top_logprobs"]
