@@ -58,7 +58,8 @@ const char *k3cuda_last_error(void);
 int  k3cuda_device_count(int *count);
 /* Wait for all work issued on the context's stream. Returns K3CUDA_ERR_TIMEOUT when a
  * kernel's bounded device-side wait gave up (the kernel skipped its work and returned; the
- * context stays usable). With a communicator the wait runs under its deadline
+ * context stays usable), K3CUDA_ERR_ARG when a kernel met an entry of a device-side table that it
+ * could not take (k3cuda_token_batch). With a communicator the wait runs under its deadline
  * (k3cuda_comm_set_timeout) and ends the communicator on a peer's failure. */
 int  k3cuda_sync(k3cuda_ctx *ctx);
 /* Bound of every device-side wait (mbarrier, peer flag) in this context's kernels, in SM
@@ -241,6 +242,95 @@ int k3cuda_mla_attend(k3cuda_ctx *ctx, void *out, int out_dtype, const void *q_n
 int k3cuda_mla_cache_append(k3cuda_ctx *ctx, void *latent, void *rope, const float *ct,
                             const float *kv_a_norm, float eps, int seq, int pos0, int T,
                             int n_cache, int cap, int dl, int dr);
+
+/* --------------------------------------- drafted tokens over a paged latent cache */
+/* A latent cache cut into pages: sequence b's position p is row p % page_size of page
+ * page_table[b][p / page_size]. latent d [n_pages][page_size][512] bf16, rope d
+ * [n_pages][page_size][64] bf16, page_table d [B][max_pages]. page_size is a power of two, 8 or
+ * more. No counterpart in the reference (one contiguous cache per process). */
+typedef struct {
+    void      *latent, *rope;
+    const int *page_table;
+    int        n_pages, page_size, max_pages;
+} k3cuda_paged_cache;
+
+/* The new tokens of B sequences, packed: sequence b has cu_tokens[b+1] - cu_tokens[b] of them
+ * (none is allowed), rows cu_tokens[b].. of the T rows of every per-token array, and cache
+ * positions ctx_lens[b].. behind its ctx_lens[b] cached rows (0 is allowed). ctx_lens d [B],
+ * cu_tokens d [B + 1], rising, cu_tokens[B] <= T. Rows from cu_tokens[B] on are padding: they are
+ * neither read nor written.
+ *
+ * page_table, ctx_lens and cu_tokens are DEVICE arrays, read when the kernels run: a captured
+ * graph replays with what they hold then. The kernels check them. A sequence that breaks a rule
+ * above is left out (its rows stay as they were) and a page number outside [0, n_pages) reads as
+ * page 0 (and is not written); either way the next k3cuda_sync returns K3CUDA_ERR_ARG. */
+typedef struct {
+    const int *ctx_lens, *cu_tokens;
+    int        B, T;
+} k3cuda_token_batch;
+
+/* Pairs of the position rotation: (i, i + dr/2) or (2 i, 2 i + 1). */
+enum { K3CUDA_ROPE_HALF = 0, K3CUDA_ROPE_INTERLEAVED = 1 };
+
+/* Append the new tokens to the paged cache and make their queries ready, in one launch. For token
+ * t, at cache position c of sequence b and rotation position p = positions[t] (positions d [T];
+ * NULL: p = c; drafts of one depth share a p):
+ *     latent row = bf16(RMSNorm(ct[t][0:dl]) * kv_a_norm)      rope row = bf16(R_p ct[t][dl:dl+dr])
+ *     q_nope[t][h] = bf16(q[t][h][0:dn])                 q_rope[t][h] = bf16(R_p q[t][h][dn:dn+dr])
+ * R_p turns pair i by the angle p * inv_freq[i] (inv_freq d [dr/2] fp32; the angle is formed and
+ * reduced in 64 bits). inv_freq NULL: no rotation, as the reference (src/core/k3_ops.c:363-366).
+ *   ct d [T][ct_stride], q d [T][q_stride] (rows of H*(dn+dr) values; strides in elements, rows
+ *   16-byte aligned) in io_dtype; q_nope d [T][H][dn], q_rope d [T][H][dr] bf16. H == 0 (q NULL)
+ *   appends only.
+ * The pages that new rows fall on belong to one sequence each. Supported: dn == 128, dr == 64,
+ * dl == 512, H <= 128. */
+int k3cuda_mla_paged_append(k3cuda_ctx *ctx, const k3cuda_paged_cache *cache,
+                            const k3cuda_token_batch *batch, const void *ct, long long ct_stride,
+                            const void *q, long long q_stride, void *q_nope, void *q_rope,
+                            int io_dtype, int H, const float *kv_a_norm, float eps,
+                            const float *inv_freq, const int *positions, int rope_style, int dn,
+                            int dr, int dl);
+
+/* Attention of every new token over its sequence's cached positions and the drafts it descends
+ * from (k3cuda_mla_decode's absorbed form over the paged cache). Token i of sequence b sees
+ * positions 0 .. ctx_lens[b]-1 and the position ctx_lens[b] + j of draft j of the same sequence
+ * where bit j of its word is set.
+ *   tree_mask  d [T] 64-bit words (a token that sees itself has its own bit set); NULL: drafts in
+ *              a row, each sees itself and those before it
+ *   out        d [T][H][dv] out_dtype; q_nope d [T][H][dn], q_rope d [T][H][dr] bf16
+ *   w_uk       d [H][dn][dl] bf16;  w_uv d [H][dv][dl] bf16
+ * At most K3CUDA_MAX_DRAFTS new tokens per sequence. A token that sees nothing (no cached row,
+ * no bit) gives zeros. What hidden or unwritten cache rows hold does not matter, infinities and
+ * NaN included; a visible draft row that holds one gives NaN. Supported: dn == dv == 128,
+ * dr == 64, dl == 512, H <= 128. workspace d: k3cuda_mla_tree_attend_workspace() bytes, 256-byte
+ * aligned, used by one call at a time. */
+#define K3CUDA_MAX_DRAFTS 64
+int k3cuda_mla_tree_attend_workspace(int B, int T, int H, int dl, int dv, size_t *bytes);
+int k3cuda_mla_tree_attend(k3cuda_ctx *ctx, void *out, int out_dtype, const void *q_nope,
+                           const void *q_rope, const k3cuda_paged_cache *cache,
+                           const k3cuda_token_batch *batch, const unsigned long long *tree_mask,
+                           const void *w_uk, const void *w_uv, int H, int dn, int dr, int dl,
+                           int dv, float scale, void *workspace, size_t workspace_bytes);
+
+/* What the model says of given tokens: from logits d [T][row_stride] (V valid values per row, in
+ * io_dtype; row_stride in elements), with p = softmax of the row,
+ *   logprobs      d [T][G]  log p[tokens[t][g]]   (tokens d [T][G]; -inf for a number outside
+ *                           [0, V), which marks an unused place; G == 0: none)
+ *   entropy       d [T]     -sum p log p, or NULL
+ *   top_ids, top_logprobs  d [T][K]  the K likeliest tokens, likeliest first, equal logits in the
+ *                           order of their numbers; places past the last token with a logit above
+ *                           -inf hold -1 and -inf (K == 0: none)
+ * in one pass over the logits, sums in fp32. A logit of -inf is a token that cannot come. A row
+ * that holds a NaN or +inf, or nothing but -inf, has no distribution: NaN, ids -1.
+ * K <= K3CUDA_MAX_TOP, V >= 1, any alignment of the rows to their element size. workspace d:
+ * k3cuda_token_logprobs_workspace() bytes (may be 0), 256-byte aligned, used by one call at a
+ * time. */
+#define K3CUDA_MAX_TOP 32
+int k3cuda_token_logprobs_workspace(int T, int V, int K, size_t *bytes);
+int k3cuda_token_logprobs(k3cuda_ctx *ctx, const void *logits, int io_dtype, long long row_stride,
+                          int T, int V, const int *tokens, int G, float *logprobs, float *entropy,
+                          int K, int *top_ids, float *top_logprobs, void *workspace,
+                          size_t workspace_bytes);
 
 /* ------------------------------------------------------- MLA layer forward */
 /* Device weights of one MLA layer, field for field K3MlaW (include/k3/k3.h:203-210):

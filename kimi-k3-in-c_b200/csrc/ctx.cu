@@ -7,6 +7,7 @@
 #include <mutex>
 
 #include "internal.cuh"
+#include "paged.cuh"
 #include "sm100.cuh"
 
 namespace k3 {
@@ -64,6 +65,17 @@ int set_smem(const void *func, int bytes) {
     K3_CUDA_TRY(cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
     if (n < 128) tab[n++] = Ent{func, dev, bytes};
     return K3CUDA_OK;
+}
+
+static const char *paged_error_text(unsigned code) {
+    switch (code) {
+        case PAGED_OFFSETS: return "cu_tokens falls, is negative or ends past the token rows";
+        case PAGED_LENGTH: return "ctx_lens holds a negative length";
+        case PAGED_DRAFTS: return "a sequence has more new tokens than the call takes";
+        case PAGED_TABLE: return "a sequence's rows pass the end of its page table";
+        case PAGED_PAGE: return "page_table names a page outside the cache";
+    }
+    return "a device-side table holds a bad entry";
 }
 
 constexpr int PIN_SLOTS = 16;
@@ -197,13 +209,14 @@ int k3cuda_sync(k3cuda_ctx *ctx) {
         if (rc) return rc;
     }
     K3_CUDA_TRY(cudaStreamSynchronize(ctx->stream));
-    // a kernel whose bounded wait gave up leaves its code in the error word
-    unsigned code = 0;
-    K3_CUDA_TRY(cudaMemcpy(&code, ctx->err_word, sizeof code, cudaMemcpyDeviceToHost));
-    if (code) {
-        K3_CUDA_TRY(cudaMemset(ctx->err_word, 0, sizeof code));
-        return set_error(K3CUDA_ERR_TIMEOUT, "a device-side wait timed out (code 0x%x)", code);
-    }
+    // a kernel whose bounded wait gave up leaves its code in word 0 of the error block, one that
+    // met a bad entry in a device-side table leaves its in word 1
+    unsigned code[2] = {0, 0};
+    K3_CUDA_TRY(cudaMemcpy(code, ctx->err_word, sizeof code, cudaMemcpyDeviceToHost));
+    if (code[0] || code[1]) K3_CUDA_TRY(cudaMemset(ctx->err_word, 0, sizeof code));
+    if (code[0])
+        return set_error(K3CUDA_ERR_TIMEOUT, "a device-side wait timed out (code 0x%x)", code[0]);
+    if (code[1]) return set_error(K3CUDA_ERR_ARG, "%s", paged_error_text(code[1]));
     return K3CUDA_OK;
 }
 

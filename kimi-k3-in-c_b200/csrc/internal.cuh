@@ -16,7 +16,8 @@ struct k3cuda_ctx {
     long long launches;
     void *flush_buf;
     size_t flush_bytes;
-    unsigned int *err_word;     // device word set by bounded waits that gave up
+    unsigned int *err_word;     // device block: word 0 set by bounded waits that gave up, word 1
+                                // by kernels that met a bad table entry (paged.cuh)
     // NCCL (opaque; see comm.cu)
     void *nccl_comm;
     int nranks, rank;
@@ -80,6 +81,12 @@ int mla_attend_kvb(k3cuda_ctx *ctx, float *acc, const void *q_nope, const void *
                    const void *latent, const void *rope, const void *kv_b, int T, int cached,
                    int cap, int H, float scale, void *workspace, size_t workspace_bytes);
 size_t mla_attend_kvb_workspace(int T, int cached, int H);
+
+// Paged cache and token batch of a call (mla_paged.cu): the checks that the host can make, and
+// the view that kernels take.
+struct PagedView;
+int paged_args_ok(const char *what, const k3cuda_paged_cache *c, const k3cuda_token_batch *b);
+PagedView paged_view(const k3cuda_paged_cache *c, const k3cuda_token_batch *b);
 
 // Host -> device copy of a small per-call table on the context's stream without the
 // stream synchronisation a pageable source may cost: the bytes go through a slot of a

@@ -21,6 +21,8 @@ GPU_LIB_PATH = os.path.join(HERE, "libk3gpu.so")
 OK, ERR_ARG, ERR_CUDA, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_NCCL, ERR_TIMEOUT, ERR_STATE = range(8)
 F32, BF16 = 0, 1
 GATE_LOG, GATE_ALPHA = 0, 1
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+MAX_DRAFTS, MAX_TOP = 64, 32       # K3CUDA_MAX_DRAFTS, K3CUDA_MAX_TOP
 MAX_EVENTS = 64
 NOALLOC_SCRATCH_BYTES = 64 << 20   # K3CUDA_NOALLOC_SCRATCH_BYTES
 
@@ -65,6 +67,14 @@ SIGNATURES = {
     "k3cuda_mla_attend": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _ip, _ip, _i, _i, _i,
                                _i, _i, _i, _i, _i, _f, _vp, _sz]),
     "k3cuda_mla_cache_append": (_i, [_vp, _vp, _vp, _vp, _vp, _f, _i, _i, _i, _i, _i, _i, _i]),
+    "k3cuda_mla_paged_append": (_i, [_vp, _vp, _vp, _vp, C.c_longlong, _vp, C.c_longlong, _vp, _vp,
+                                     _i, _i, _vp, _f, _vp, _vp, _i, _i, _i, _i]),
+    "k3cuda_mla_tree_attend_workspace": (_i, [_i, _i, _i, _i, _i, C.POINTER(_sz)]),
+    "k3cuda_mla_tree_attend": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i,
+                                    _i, _i, _f, _vp, _sz]),
+    "k3cuda_token_logprobs_workspace": (_i, [_i, _i, _i, C.POINTER(_sz)]),
+    "k3cuda_token_logprobs": (_i, [_vp, _vp, _i, C.c_longlong, _i, _i, _vp, _i, _vp, _vp, _i, _vp,
+                                   _vp, _vp, _sz]),
     "k3cuda_mla_layer_workspace": (_i, [_i, _i, _i, _i, _i, _i, C.POINTER(_sz)]),
     "k3cuda_mla_layer": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _vp,
                               _i, _i, _vp, _sz]),
@@ -103,6 +113,17 @@ class MlaWeights(C.Structure):
     """k3cuda_mla_weights: device pointers of one MLA layer, in K3MlaW's field order."""
     _fields_ = [("q_a", _vp), ("q_b", _vp), ("kv_a", _vp), ("kv_b", _vp), ("o", _vp),
                 ("g", _vp), ("q_a_norm", _vp), ("kv_a_norm", _vp), ("wdt", _i)]
+
+
+class PagedCache(C.Structure):
+    """k3cuda_paged_cache: device pointers of a paged latent cache and its page table."""
+    _fields_ = [("latent", _vp), ("rope", _vp), ("page_table", _vp), ("n_pages", _i),
+                ("page_size", _i), ("max_pages", _i)]
+
+
+class TokenBatch(C.Structure):
+    """k3cuda_token_batch: device pointers of the new tokens' cache lengths and offsets."""
+    _fields_ = [("ctx_lens", _vp), ("cu_tokens", _vp), ("B", _i), ("T", _i)]
 
 
 class Cfg(C.Structure):
@@ -385,6 +406,38 @@ class Context:
         check(lib().k3cuda_mla_cache_append(self.h, _ptr(latent), _ptr(rope), _ptr(ct),
                                             _ptr(kv_a_norm), float(eps), int(seq), int(pos0),
                                             int(T), int(n_cache), int(cap), 512, 64))
+
+    # drafted tokens over a paged latent cache ---------------------------------------
+    def mla_paged_append(self, cache, batch, ct, kv_a_norm, eps, q=None, q_nope=None, q_rope=None,
+                         H=0, positions=None, inv_freq=None, rope_style=ROPE_HALF, io_dtype=F32,
+                         ct_stride=576, q_stride=None):
+        """cache: PagedCache, batch: TokenBatch; a program keeps them between calls."""
+        check(lib().k3cuda_mla_paged_append(
+            self.h, C.byref(cache), C.byref(batch), _ptr(ct), int(ct_stride), _ptr(q),
+            int(H * 192 if q_stride is None else q_stride), _ptr(q_nope), _ptr(q_rope),
+            int(io_dtype), int(H), _ptr(kv_a_norm), float(eps), _ptr(inv_freq), _ptr(positions),
+            int(rope_style), 128, 64, 512))
+
+    def mla_tree_attend_workspace(self, B, T, H) -> int:
+        return _ws_query(lib().k3cuda_mla_tree_attend_workspace, int(B), int(T), int(H), 512, 128)
+
+    def mla_tree_attend(self, out, q_nope, q_rope, cache, batch, w_uk, w_uv, H, scale, workspace,
+                        workspace_bytes, tree_mask=None, out_dtype=F32):
+        check(lib().k3cuda_mla_tree_attend(
+            self.h, _ptr(out), int(out_dtype), _ptr(q_nope), _ptr(q_rope), C.byref(cache),
+            C.byref(batch), _ptr(tree_mask), _ptr(w_uk), _ptr(w_uv), int(H), 128, 64, 512, 128,
+            float(scale), _ptr(workspace), int(workspace_bytes)))
+
+    def token_logprobs_workspace(self, T, V, K=0) -> int:
+        return _ws_query(lib().k3cuda_token_logprobs_workspace, int(T), int(V), int(K))
+
+    def token_logprobs(self, logits, T, V, tokens, G, logprobs, workspace=None, workspace_bytes=0,
+                       entropy=None, K=0, top_ids=None, top_logprobs=None, io_dtype=F32,
+                       row_stride=None):
+        check(lib().k3cuda_token_logprobs(
+            self.h, _ptr(logits), int(io_dtype), int(V if row_stride is None else row_stride),
+            int(T), int(V), _ptr(tokens), int(G), _ptr(logprobs), _ptr(entropy), int(K),
+            _ptr(top_ids), _ptr(top_logprobs), _ptr(workspace), int(workspace_bytes)))
 
     def mla_layer_workspace(self, T, E, H, q_lora, cached, wdt) -> int:
         return _ws_query(lib().k3cuda_mla_layer_workspace, int(T), int(E), int(H), int(q_lora),
