@@ -82,6 +82,14 @@ int mla_attend_kvb(k3cuda_ctx *ctx, float *acc, const void *q_nope, const void *
                    int cap, int H, float scale, void *workspace, size_t workspace_bytes);
 size_t mla_attend_kvb_workspace(int T, int cached, int H);
 
+// The per-head products around the absorbed attention (mla_decode.cu).
+int mla_absorb(k3cuda_ctx *ctx, __nv_bfloat16 *qlat, int pitch, const void *q_nope,
+               const void *q_rope, const void *w_uk, int uk_head_rows, int B, int H);
+int mla_project(k3cuda_ctx *ctx, void *out, int out_dtype, const __nv_bfloat16 *olat2,
+                const float *rowsum, const int *keep, const void *w_uv, int uv_head_rows, int B,
+                int H);
+constexpr float MLA_RESCALE_LOG2 = 8.f;    // lazy rescale threshold (factor 256)
+
 // Paged cache and token batch of a call (mla_paged.cu): the checks that the host can make, and
 // the view that kernels take.
 struct PagedView;

@@ -82,7 +82,6 @@ constexpr int MLA_PART = MLA_DL + 4;       // floats per (segment, head): o_lat,
 // TMEM columns: S [0, 64), this rank's query half [64, 224) (two bf16 per column),
 // O [256, 512)
 constexpr int MLA_TM_S = 0, MLA_TM_Q = 64, MLA_TM_O = 256, MLA_TM_COLS = 512;
-constexpr float MLA_RESCALE_LOG2 = 8.f;    // lazy rescale threshold (factor 256)
 
 __device__ __forceinline__ float bf(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
 
@@ -111,7 +110,8 @@ struct HeadGemmMaps {
 // W_UK block is split over two CTAs, and two CTAs (97 KB of shared memory each) share an SM.
 __global__ void __launch_bounds__(128, 2)
 mla_q_absorb_tc(const __grid_constant__ HeadGemmMaps maps, const __nv_bfloat16 *__restrict__ q_rope,
-                __nv_bfloat16 *__restrict__ qlat, int B, int H, unsigned *__restrict__ err) {
+                __nv_bfloat16 *__restrict__ qlat, int pitch, int B, int H,
+                unsigned *__restrict__ err) {
     extern __shared__ uint8_t smraw[];
     uint8_t *sm = (uint8_t *)(((uintptr_t)smraw + 1023) & ~(uintptr_t)1023);
     uint8_t *sA = sm;              // 2 K-blocks x [128 b][128 B]
@@ -165,15 +165,15 @@ mla_q_absorb_tc(const __grid_constant__ HeadGemmMaps maps, const __nv_bfloat16 *
                     const __nv_bfloat162 t2 = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
                     pk[i] = *reinterpret_cast<const uint32_t *>(&t2);
                 }
-                uint4 *dst = reinterpret_cast<uint4 *>(qlat + ((size_t)b * MLA_HP + h) * MLA_QW +
-                                                       256 * z + c);
+                uint4 *dst = reinterpret_cast<uint4 *>(qlat + ((size_t)b * pitch + h) * MLA_QW + 256 * z +
+                                                       c);
                 dst[0] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
                 dst[1] = make_uint4(pk[4], pk[5], pk[6], pk[7]);
             }
         }
         if (b < B && z == 0) {
             const uint4 *src = reinterpret_cast<const uint4 *>(q_rope + ((size_t)b * H + h) * MLA_DR);
-            uint4 *dst = reinterpret_cast<uint4 *>(qlat + ((size_t)b * MLA_HP + h) * MLA_QW + MLA_DL);
+            uint4 *dst = reinterpret_cast<uint4 *>(qlat + ((size_t)b * pitch + h) * MLA_QW + MLA_DL);
 #pragma unroll
             for (int i = 0; i < MLA_DR / 8; i++) dst[i] = src[i];
         }
@@ -186,9 +186,19 @@ mla_q_absorb_tc(const __grid_constant__ HeadGemmMaps maps, const __nv_bfloat16 *
     }
 }
 
+// What o_lat's row is divided by on the way out: its softmax sum where the caller left that to
+// the projection (0 for a row that saw nothing, whose o_lat is 0 too), else nothing.
+__device__ __forceinline__ float row_factor(const float *rowsum, size_t row) {
+    if (!rowsum) return 1.f;
+    const float l = rowsum[row];
+    return l == 0.f ? 0.f : 1.f / l;
+}
+
+// rowsum: see row_factor; keep [B]: rows of 0 are not stored (NULL: every row is)
 template <typename OUT>
 __global__ void __launch_bounds__(128, 2)
 mla_project_tc(const __grid_constant__ HeadGemmMaps maps, OUT *__restrict__ out, int B, int H,
+               const float *__restrict__ rowsum, const int *__restrict__ keep,
                unsigned *__restrict__ err) {
     // K blocks of 64 (hi 0..7, lo 8..15); each stage holds one A block (o_lat rows) and the
     // W_UV block it meets, so a CTA needs 97 KB of shared memory and two share an SM
@@ -250,13 +260,16 @@ mla_project_tc(const __grid_constant__ HeadGemmMaps maps, OUT *__restrict__ out,
     tc_fence_after();
     const int b = b0 + 32 * warp + (tid & 31);
     if (ok) {
+        const bool st = b < B && (!keep || keep[b]);
+        const float f = st ? row_factor(rowsum, (size_t)b * H + h) : 0.f;
         for (int c = 0; c < 128; c += 16) {
             float v[16];
             tmem_ld16(tb + ((uint32_t)(32 * warp) << 16) + c, v);
             tmem_wait_ld();
-            if (b < B)
+            if (st)
 #pragma unroll
-                for (int i = 0; i < 16; i++) io<OUT>::st(out + ((size_t)b * H + h) * MLA_DV + c + i, v[i]);
+                for (int i = 0; i < 16; i++)
+                    io<OUT>::st(out + ((size_t)b * H + h) * MLA_DV + c + i, v[i] * f);
         }
     }
     tc_fence_before();
@@ -672,7 +685,7 @@ template <int NB>
 __global__ void __launch_bounds__(256)
 mla_q_absorb_small(const __nv_bfloat16 *__restrict__ q_nope,
                    const __nv_bfloat16 *__restrict__ q_rope, const __nv_bfloat16 *__restrict__ w_uk,
-                   long long uk_head_elems, __nv_bfloat16 *__restrict__ qlat, int B, int H) {
+                   long long uk_head_elems, __nv_bfloat16 *__restrict__ qlat, int pitch, int B, int H) {
     __shared__ float qs[NB][MLA_DN];
     __shared__ float red[8][NB][128];
     pdl_trigger();
@@ -689,11 +702,11 @@ mla_q_absorb_small(const __nv_bfloat16 *__restrict__ q_nope,
     if (h >= H) {
         // a padding head of the MMA's M: its query row must score zero
         for (int e = tid; e < B * 128; e += 256)
-            qlat[((size_t)(e >> 7) * MLA_HP + h) * MLA_QW + 128 * z + (e & 127)] =
+            qlat[((size_t)(e >> 7) * pitch + h) * MLA_QW + 128 * z + (e & 127)] =
                 __float2bfloat16_rn(0.f);
         if (z == 0)
             for (int e = tid; e < B * MLA_DR; e += 256)
-                qlat[((size_t)(e / MLA_DR) * MLA_HP + h) * MLA_QW + MLA_DL + e % MLA_DR] =
+                qlat[((size_t)(e / MLA_DR) * pitch + h) * MLA_QW + MLA_DL + e % MLA_DR] =
                     __float2bfloat16_rn(0.f);
         return;
     }
@@ -740,11 +753,11 @@ mla_q_absorb_small(const __nv_bfloat16 *__restrict__ q_nope,
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < 8; w++) v += red[w][b][c];
-        qlat[((size_t)b * MLA_HP + h) * MLA_QW + 128 * z + c] = __float2bfloat16_rn(v);
+        qlat[((size_t)b * pitch + h) * MLA_QW + 128 * z + c] = __float2bfloat16_rn(v);
     }
     if (z == 0)
         for (int e = tid; e < B * MLA_DR; e += 256)
-            qlat[((size_t)(e / MLA_DR) * MLA_HP + h) * MLA_QW + MLA_DL + e % MLA_DR] =
+            qlat[((size_t)(e / MLA_DR) * pitch + h) * MLA_QW + MLA_DL + e % MLA_DR] =
                 q_rope[((size_t)(e / MLA_DR) * H + h) * MLA_DR + e % MLA_DR];
 }
 
@@ -754,7 +767,8 @@ mla_q_absorb_small(const __nv_bfloat16 *__restrict__ q_nope,
 template <typename OUT>
 __global__ void __launch_bounds__(256)
 mla_project_small(const __nv_bfloat16 *__restrict__ olat2, const __nv_bfloat16 *__restrict__ w_uv,
-                  long long uv_head_elems, OUT *__restrict__ out, int B, int H) {
+                  long long uv_head_elems, OUT *__restrict__ out, int B, int H,
+                  const float *__restrict__ rowsum, const int *__restrict__ keep) {
     // o_lat rows with one pad float after every 16: lane l reads elements 16 l .. 16 l + 15,
     // at 17 l .. 17 l + 15, so the 32 lanes of a read fall in 32 different banks
     constexpr int OSW = MLA_DL + MLA_DL / 16;
@@ -795,7 +809,9 @@ mla_project_small(const __nv_bfloat16 *__restrict__ olat2, const __nv_bfloat16 *
             for (int x = 0; x < 16; x++) v = fmaf(os[b][17 * lane + x], wf[x], v);
 #pragma unroll
             for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            if (lane == 0) io<OUT>::st(out + ((size_t)b * H + h) * MLA_DV + j0 + r, v);
+            if (lane == 0 && (!keep || keep[b]))
+                io<OUT>::st(out + ((size_t)b * H + h) * MLA_DV + j0 + r,
+                            v * row_factor(rowsum, (size_t)b * H + h));
         }
     }
 }
@@ -984,6 +1000,82 @@ static size_t mla_ws_bound(int B, int H) {
     return mla_ws_bytes(p, B, H);
 }
 
+// qlat[b * pitch + h] = [W_UK[h]^T q_nope[b][h] | q_rope[b][h]] (bf16, MLA_QW wide) for B
+// queries; with pitch == MLA_HP and a few queries also zeroes the rows of heads H .. MLA_HP - 1.
+int mla_absorb(k3cuda_ctx *ctx, __nv_bfloat16 *qlat, int pitch, const void *q_nope,
+               const void *q_rope, const void *w_uk, int uk_head_rows, int B, int H) {
+    const CUtensorMapDataType BF = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const __nv_bfloat16 *qn = (const __nv_bfloat16 *)q_nope, *qr = (const __nv_bfloat16 *)q_rope,
+                        *wk = (const __nv_bfloat16 *)w_uk;
+    if (B <= MLA_SMALL_B) {
+        const dim3 g(pitch, MLA_DL / 128), blk(256);
+        const long long uk = (long long)uk_head_rows * MLA_DL;
+        const char *nm = "mla_q_absorb_small";
+        if (B <= 1)
+            return launch_pdl(ctx, ctx->stream, nm, mla_q_absorb_small<1>, g, blk, 0, qn, qr, wk,
+                              uk, qlat, pitch, B, H);
+        if (B <= 2)
+            return launch_pdl(ctx, ctx->stream, nm, mla_q_absorb_small<2>, g, blk, 0, qn, qr, wk,
+                              uk, qlat, pitch, B, H);
+        if (B <= 4)
+            return launch_pdl(ctx, ctx->stream, nm, mla_q_absorb_small<4>, g, blk, 0, qn, qr, wk,
+                              uk, qlat, pitch, B, H);
+        return launch_pdl(ctx, ctx->stream, nm, mla_q_absorb_small<8>, g, blk, 0, qn, qr, wk, uk,
+                          qlat, pitch, B, H);
+    }
+    HeadGemmMaps maps;
+    int rc = make_tmap_3d(&maps.a, q_nope, BF, 2, MLA_DN, H, B, MLA_DN * 2,
+                          (uint64_t)H * MLA_DN * 2, 64, 1, 128);
+    if (!rc)
+        rc = make_tmap_3d(&maps.b, w_uk, BF, 2, MLA_DL, MLA_DN, H, MLA_DL * 2,
+                          (uint64_t)uk_head_rows * MLA_DL * 2, 64, 64, 1);
+    if (rc) return rc;
+    const int smem = 2 * 16384 + 8 * 8192 + 1024;
+    if ((rc = set_smem(mla_q_absorb_tc, smem))) return rc;
+    const dim3 grid(H, (B + 127) / 128, 2);  // two 256-column halves of q_lat per head
+    mla_q_absorb_tc<<<grid, 128, smem, ctx->stream>>>(maps, qr, qlat, pitch, B, H, ctx->err_word);
+    return after_launch(ctx, "mla_q_absorb_tc");
+}
+
+// out[b][h] = W_UV[h] o_lat[b][h] / rowsum[b][h], o_lat as bf16 hi/lo pairs [B][H][2 MLA_DL];
+// rowsum and keep as mla_project_tc.
+int mla_project(k3cuda_ctx *ctx, void *out, int out_dtype, const __nv_bfloat16 *olat2,
+                const float *rowsum, const int *keep, const void *w_uv, int uv_head_rows, int B,
+                int H) {
+    const CUtensorMapDataType BF = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const bool bf = out_dtype == K3CUDA_BF16;
+    if (B <= MLA_SMALL_B) {
+        const dim3 grid(H, MLA_DV / 16), blk(256);
+        const long long uv = (long long)uv_head_rows * MLA_DL;
+        const __nv_bfloat16 *wu = (const __nv_bfloat16 *)w_uv;
+        const char *nm = "mla_project_small";
+        if (bf)
+            return launch_pdl(ctx, ctx->stream, nm, mla_project_small<__nv_bfloat16>, grid, blk, 0,
+                              olat2, wu, uv, (__nv_bfloat16 *)out, B, H, rowsum, keep);
+        return launch_pdl(ctx, ctx->stream, nm, mla_project_small<float>, grid, blk, 0, olat2, wu,
+                          uv, (float *)out, B, H, rowsum, keep);
+    }
+    HeadGemmMaps maps;
+    int rc = make_tmap_3d(&maps.a, olat2, BF, 2, 2 * MLA_DL, H, B, 2 * MLA_DL * 2,
+                          (uint64_t)H * 2 * MLA_DL * 2, 64, 1, 128);
+    if (!rc)
+        rc = make_tmap_3d(&maps.b, w_uv, BF, 2, MLA_DL, MLA_DV, H, MLA_DL * 2,
+                          (uint64_t)uv_head_rows * MLA_DL * 2, 64, 128, 1);
+    if (rc) return rc;
+    const dim3 grid(H, (B + 127) / 128);
+    const int smem = 3 * 2 * 16384 + 1024;
+    if (bf) {
+        if ((rc = set_smem(mla_project_tc<__nv_bfloat16>, smem))) return rc;
+        mla_project_tc<__nv_bfloat16><<<grid, 128, smem, ctx->stream>>>(
+            maps, (__nv_bfloat16 *)out, B, H, rowsum, keep, ctx->err_word);
+    } else {
+        if ((rc = set_smem(mla_project_tc<float>, smem))) return rc;
+        mla_project_tc<float><<<grid, 128, smem, ctx->stream>>>(maps, (float *)out, B, H, rowsum,
+                                                                keep, ctx->err_word);
+    }
+    return after_launch(ctx, "mla_project_tc");
+}
+
 }  // namespace k3
 
 using namespace k3;
@@ -1081,65 +1173,23 @@ static int mla_run(k3cuda_ctx *ctx, void *out, int out_dtype, const void *q_nope
         put(d_row0, row0.data(), (size_t)B * sizeof(int));
         if ((rc = stage_h2d(ctx, workspace, img.data(), tbytes))) return rc;
     }
-    const bool small = B <= MLA_SMALL_B;  // the small absorb kernel zeroes the padded rows
-    if (H < MLA_HP && !small)  // the padded query rows must score zero
+    if (H < MLA_HP && B > MLA_SMALL_B)  // the padded query rows must score zero (the absorption
+                                        // of a few sequences writes them itself)
         K3_CUDA_TRY(cudaMemset2DAsync(qlat + (size_t)H * MLA_QW, (size_t)MLA_HP * MLA_QW * 2, 0,
                                       (size_t)(MLA_HP - H) * MLA_QW * 2, (size_t)B, ctx->stream));
 
     const CUtensorMapDataType BF = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    HeadGemmMaps qmaps, pmaps;
     MlaMaps maps;
-    rc = make_tmap_3d(&qmaps.a, q_nope, BF, 2, MLA_DN, H, B, MLA_DN * 2, (uint64_t)H * MLA_DN * 2,
-                      64, 1, 128);
-    if (!rc)
-        rc = make_tmap_3d(&qmaps.b, w_uk, BF, 2, MLA_DL, MLA_DN, H, MLA_DL * 2,
-                          (uint64_t)uk_head_rows * MLA_DL * 2, 64, 64, 1);
-    if (!rc)
-        rc = make_tmap_2d(&maps.lat, latent, BF, 2, MLA_DL, (uint64_t)n_cache * cap, MLA_DL * 2,
-                          64, MLA_TILE);
+    rc = make_tmap_2d(&maps.lat, latent, BF, 2, MLA_DL, (uint64_t)n_cache * cap, MLA_DL * 2, 64,
+                      MLA_TILE);
     if (!rc)
         rc = make_tmap_2d(&maps.rope, rope, BF, 2, MLA_DR, (uint64_t)n_cache * cap, MLA_DR * 2,
                           64, MLA_TILE);
-    if (!rc)
-        rc = make_tmap_3d(&pmaps.a, olat2, BF, 2, 2 * MLA_DL, H, B, 2 * MLA_DL * 2,
-                          (uint64_t)H * 2 * MLA_DL * 2, 64, 1, 128);
-    if (!rc)
-        rc = make_tmap_3d(&pmaps.b, w_uv, BF, 2, MLA_DL, MLA_DV, H, MLA_DL * 2,
-                          (uint64_t)uv_head_rows * MLA_DL * 2, 64, 128, 1);
     if (rc) return rc;
     K3_ARG_CHECK(aligned(q_nope, 16) && aligned(q_rope, 16) && aligned(w_uk, 16) &&
                      aligned(w_uv, 16),
                  "MLA inputs must be 16-byte aligned");
-
-    const dim3 hgrid(H, (B + 127) / 128);
-    if (small) {
-        const dim3 g(MLA_HP, MLA_DL / 128);
-        const __nv_bfloat16 *qn = (const __nv_bfloat16 *)q_nope, *qr = (const __nv_bfloat16 *)q_rope,
-                            *wk = (const __nv_bfloat16 *)w_uk;
-        const long long uk = (long long)uk_head_rows * MLA_DL;
-        const char *nm = "mla_q_absorb_small";
-        const dim3 blk(256);
-        if (B <= 1)
-            rc = launch_pdl(ctx, ctx->stream, nm, mla_q_absorb_small<1>, g, blk, 0, qn, qr, wk, uk,
-                            qlat, B, H);
-        else if (B <= 2)
-            rc = launch_pdl(ctx, ctx->stream, nm, mla_q_absorb_small<2>, g, blk, 0, qn, qr, wk, uk,
-                            qlat, B, H);
-        else if (B <= 4)
-            rc = launch_pdl(ctx, ctx->stream, nm, mla_q_absorb_small<4>, g, blk, 0, qn, qr, wk, uk,
-                            qlat, B, H);
-        else
-            rc = launch_pdl(ctx, ctx->stream, nm, mla_q_absorb_small<8>, g, blk, 0, qn, qr, wk, uk,
-                            qlat, B, H);
-    } else {
-        const int qsmem = 2 * 16384 + 8 * 8192 + 1024;
-        if (int rc_ = set_smem(mla_q_absorb_tc, qsmem)) return rc_;
-        const dim3 qgrid(H, (B + 127) / 128, 2);  // two 256-column halves of q_lat per head
-        mla_q_absorb_tc<<<qgrid, 128, qsmem, ctx->stream>>>(qmaps, (const __nv_bfloat16 *)q_rope,
-                                                            qlat, B, H, ctx->err_word);
-        rc = after_launch(ctx, "mla_q_absorb_tc");
-    }
-    if (rc) return rc;
+    if ((rc = mla_absorb(ctx, qlat, MLA_HP, q_nope, q_rope, w_uk, uk_head_rows, B, H))) return rc;
 
     if (int rc_ = set_smem(mla_attend_tc, MLA_SMEM)) return rc_;
     const float scale_log2e = scale * 1.4426950408889634f;
@@ -1152,29 +1202,7 @@ static int mla_run(k3cuda_ctx *ctx, void *out, int out_dtype, const void *q_nope
     rc = launch_pdl(ctx, ctx->stream, "mla_merge", mla_merge, dim3(H, B), dim3(128), 0,
                     (const float *)part, (const int *)d_slot0, olat2, H);
     if (rc) return rc;
-
-    if (small) {
-        const dim3 pgrid(H, MLA_DV / 16);
-        const long long uv = (long long)uv_head_rows * MLA_DL;
-        const __nv_bfloat16 *o2 = olat2, *wu = (const __nv_bfloat16 *)w_uv;
-        if (out_dtype == K3CUDA_BF16)
-            return launch_pdl(ctx, ctx->stream, "mla_project_small",
-                              mla_project_small<__nv_bfloat16>, pgrid, dim3(256), 0, o2, wu, uv,
-                              (__nv_bfloat16 *)out, B, H);
-        return launch_pdl(ctx, ctx->stream, "mla_project_small", mla_project_small<float>, pgrid,
-                          dim3(256), 0, o2, wu, uv, (float *)out, B, H);
-    }
-    const int psmem = 3 * 2 * 16384 + 1024;
-    if (out_dtype == K3CUDA_BF16) {
-        if (int rc_ = set_smem(mla_project_tc<__nv_bfloat16>, psmem)) return rc_;
-        mla_project_tc<__nv_bfloat16><<<hgrid, 128, psmem, ctx->stream>>>(
-            pmaps, (__nv_bfloat16 *)out, B, H, ctx->err_word);
-    } else {
-        if (int rc_ = set_smem(mla_project_tc<float>, psmem)) return rc_;
-        mla_project_tc<float><<<hgrid, 128, psmem, ctx->stream>>>(pmaps, (float *)out, B, H,
-                                                                  ctx->err_word);
-    }
-    return after_launch(ctx, "mla_project_tc");
+    return mla_project(ctx, out, out_dtype, olat2, nullptr, nullptr, w_uv, uv_head_rows, B, H);
 }
 
 namespace k3 {

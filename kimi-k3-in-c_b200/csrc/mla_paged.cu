@@ -200,7 +200,7 @@ int paged_args_ok(const char *what, const k3cuda_paged_cache *c, const k3cuda_to
         return set_error(K3CUDA_ERR_UNSUPPORTED,
                          "%s: page_size=%d not built (a power of two, 8 or more)", what, p);
     K3_ARG_CHECK((long long)c->n_pages * p < (1ll << 31) &&
-                     (long long)c->max_pages * p < (1ll << 31) - 64,
+                     (long long)c->max_pages * p < (1ll << 31) - 128,
                  "%s: %d (table: %d) pages of %d rows pass 32-bit row numbers", what, c->n_pages,
                  c->max_pages, p);
     K3_ARG_CHECK(c->latent && c->rope && c->page_table && b->ctx_lens && b->cu_tokens,

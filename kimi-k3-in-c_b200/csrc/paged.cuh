@@ -85,11 +85,11 @@ template <typename A, typename X> K3_HD int last_at_most(const A *a, int n, X x)
     return lo;
 }
 
-// Which of the 64 positions of tile t (positions 64 t .. 64 t + 63) a draft sees, as bits: every
-// cached position (below len), and the drafts j (at len + j, j < n) whose bit is set in `mask`.
-K3_HD uint64_t tree_tile_bits(uint64_t mask, int len, int n, int t) {
+// Which of the 64 positions p0 .. p0 + 63 a draft sees, as bits: every cached position (below
+// len), and the drafts j (at len + j, j < n) whose bit is set in `mask`.
+K3_HD uint64_t tree_bits(uint64_t mask, int len, int n, long long p0) {
     if (n < 64) mask &= ((uint64_t)1 << n) - 1;
-    const long long d = (long long)t * 64 - len;  // draft index of the tile's first position
+    const long long d = p0 - len;  // draft index of the first position
     if (d >= 64) return 0;
     if (d >= 0) return mask >> d;
     if (d <= -64) return ~(uint64_t)0;

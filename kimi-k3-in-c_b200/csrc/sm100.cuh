@@ -318,6 +318,18 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *v) {
     for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
 }
 
+// As tmem_ld16, 8 consecutive columns.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float *v) {
+    uint32_t r[8];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = __uint_as_float(r[i]);
+}
+
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&v)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
@@ -339,7 +351,7 @@ __device__ __forceinline__ void tmem_wait_st() {
 }
 
 // ----------------------------------------------------------------------- descriptors
-constexpr uint32_t kSw128 = 2;  // layout type: 128-byte swizzle
+constexpr uint32_t kSw128 = 2, kSw64 = 4;  // layout types: 128- and 64-byte swizzle
 
 // Shared-memory matrix descriptor (start, leading and stride byte offsets, SW128).
 __device__ __forceinline__ uint64_t sdesc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
@@ -350,6 +362,13 @@ __device__ __forceinline__ uint64_t sdesc(uint32_t saddr, uint32_t lbo, uint32_t
 // K-major SW128 operand at `saddr` (1024-aligned region of rows x 128 B): the K step of
 // 16 bf16 (or 8 tf32) is +32 B on the start address.
 __device__ __forceinline__ uint64_t sdesc_kmajor(uint32_t saddr) { return sdesc(saddr, 16, 1024); }
+
+// K-major operand of 32 bf16 per row with the 64-byte swizzle (rows x 64 B, 512-aligned region:
+// eight rows form an atom, 16-byte chunk c of row r sits at c ^ ((r >> 1) & 3)).
+__device__ __forceinline__ uint64_t sdesc_kmajor64(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | (1ull << 16) | ((uint64_t)(512 >> 4) << 32) |
+           (1ull << 46) | ((uint64_t)kSw64 << 61);
+}
 
 // MN-major SW128 operand: `mn_stride` bytes between consecutive 64-wide M/N blocks.
 __device__ __forceinline__ uint64_t sdesc_mnmajor(uint32_t saddr, uint32_t mn_stride) {
@@ -395,6 +414,15 @@ __device__ __forceinline__ void mma_commit(uint64_t *bar) {
                  : "memory");
 }
 
+// As mma_commit, arriving on the barrier at the same shared offset of every CTA in `mask`.
+__device__ __forceinline__ void mma_commit_cluster(uint64_t *bar, uint16_t mask) {
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(smem_u32(bar)),
+        "h"(mask)
+        : "memory");
+}
+
 // ---------------------------------------------------------------------------- cluster
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -427,6 +455,14 @@ __device__ __forceinline__ void st_async_v4(uint32_t raddr, float a, float b, fl
     asm volatile(
         "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::
             "r"(raddr), "f"(a), "f"(b), "f"(c), "f"(d), "r"(rbar)
+        : "memory");
+}
+
+// As st_async_v4, four bytes.
+__device__ __forceinline__ void st_async_f32(uint32_t raddr, float a, uint32_t rbar) {
+    asm volatile(
+        "st.async.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(raddr),
+        "f"(a), "r"(rbar)
         : "memory");
 }
 

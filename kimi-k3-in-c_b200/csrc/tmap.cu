@@ -88,8 +88,9 @@ int make_tmap_2d(CUtensorMap *map, const void *base, CUtensorMapDataType dtype,
     cuuint64_t strides[1] = {row_bytes};
     cuuint32_t box[2] = {box_inner, box_outer};
     cuuint32_t estr[2] = {1, 1};
-    const CUtensorMapSwizzle sw = box_inner * elem_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
-                                                                : CU_TENSOR_MAP_SWIZZLE_NONE;
+    const CUtensorMapSwizzle sw = box_inner * elem_bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                  : box_inner * elem_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                                 : CU_TENSOR_MAP_SWIZZLE_NONE;
     CUresult r = fn(map, dtype, 2, const_cast<void *>(base), dims, strides, box, estr,
                     CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

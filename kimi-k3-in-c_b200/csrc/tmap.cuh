@@ -10,7 +10,8 @@
 namespace k3 {
 
 // 2-D row-major tensor [outer][inner] of `elem_bytes` elements with `row_bytes` between
-// rows; box [box_outer][box_inner]; 128-byte swizzle when box_inner * elem_bytes == 128.
+// rows; box [box_outer][box_inner]; 128-byte (64-byte) swizzle when box_inner * elem_bytes
+// is 128 (64).
 // Returns K3CUDA_OK or an error code with the message set.
 int make_tmap_2d(CUtensorMap *map, const void *base, CUtensorMapDataType dtype,
                  uint32_t elem_bytes, uint64_t inner, uint64_t outer, uint64_t row_bytes,

@@ -221,10 +221,10 @@ int main() {
     for (int it = 0; it < 3000; it++) {
         const int n = rnd(0, 64), len = rnd(0, 300);
         const uint64_t mask = ((uint64_t)g() << 32) | g();
-        for (int t = 0; t < 7; t++) {
-            const uint64_t w = tree_tile_bits(mask, len, n, t);
+        for (int p0 = 0; p0 < 450; p0 += rnd(1, 64)) {
+            const uint64_t w = tree_bits(mask, len, n, p0);
             for (int c = 0; c < 64; c++) {
-                const int j = 64 * t + c - len;
+                const int j = p0 + c - len;
                 const bool see = j < 0 || (j < n && ((mask >> j) & 1));
                 assert(((w >> c) & 1) == (see ? 1u : 0u));
             }

@@ -652,13 +652,35 @@ def test_a_verification_step(ctx):
             host, dev, bufs = step_data(ctx, rng, p, H, V)
 
 
+class Graph:
+    """What the library issues on a context's stream, captured and replayed through the CUDA
+    runtime that it is linked against."""
+
+    def __init__(self, ctx, fn):
+        self.rt = C.CDLL("libcudart.so.12")
+        self.stream = C.c_void_p(k3cuda.lib().k3cuda_stream(ctx.h))
+        graph, self.exe = C.c_void_p(), C.c_void_p()
+        assert self.rt.cudaStreamBeginCapture(self.stream, 1) == 0   # this thread's calls
+        try:
+            fn()
+        finally:
+            rc = self.rt.cudaStreamEndCapture(self.stream, C.byref(graph))
+        assert rc == 0
+        assert self.rt.cudaGraphInstantiate(C.byref(self.exe), graph, C.c_ulonglong(0)) == 0
+        assert self.rt.cudaGraphDestroy(graph) == 0
+
+    def replay(self):
+        assert self.rt.cudaGraphLaunch(self.exe, self.stream) == 0
+
+    def close(self):
+        assert self.rt.cudaGraphExecDestroy(self.exe) == 0
+
+
 def test_captured_step_replays_with_new_lengths(ctx):
     """A captured step reads lengths, offsets and pages when it is replayed; two captured steps
     with a workspace each do not disturb one another."""
-    torch = pytest.importorskip("torch")
     rng = np.random.default_rng(21)
     H, V = 8, 1003
-    stream = torch.cuda.ExternalStream(k3cuda.lib().k3cuda_stream(ctx.h))
     parts = []
     for k in range(2):
         p = Paged(ctx, rng, [200, 90], [4, 4], 16)
@@ -666,10 +688,8 @@ def test_captured_step_replays_with_new_lengths(ctx):
         dw = ctx.upload(tree_words(rng, p.toks, "chain"))
         verify_step(ctx, p, dev, H, V, dw, bufs)   # warm: attributes are set outside the capture
         ctx.sync()
-        g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g, stream=stream, capture_error_mode="thread_local"):
-            verify_step(ctx, p, dev, H, V, dw, bufs)
-        parts.append((p, dev, bufs, dw, g))
+        parts.append((p, dev, bufs, dw,
+                      Graph(ctx, lambda: verify_step(ctx, p, dev, H, V, dw, bufs))))
     names = ("out", "lp", "ent", "ids", "tlp")
     for lens, toks in (([200, 90], [4, 4]), ([33, 0], [1, 7]), ([0, 150], [8, 0])):
         want = []
@@ -685,15 +705,15 @@ def test_captured_step_replays_with_new_lengths(ctx):
             for n in names:
                 bufs[n].zero()
         ctx.sync()
-        with torch.cuda.stream(stream):
-            for _ in range(2):
-                for part in parts:
-                    part[4].replay()
+        for _ in range(2):
+            for part in parts:
+                part[4].replay()
         ctx.sync()
         for (p, dev, bufs, dw, g), w in zip(parts, want):
             for n, a in zip(names, w):
                 assert np.array_equal(bufs[n].numpy(), a, equal_nan=True), n
-    del parts
+    for part in parts:
+        part[4].close()
 
 
 def test_two_contexts_at_once(ctx):
