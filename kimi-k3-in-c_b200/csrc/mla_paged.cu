@@ -213,8 +213,10 @@ int paged_args_ok(const char *what, const k3cuda_paged_cache *c, const k3cuda_to
 }
 
 PagedView paged_view(const k3cuda_paged_cache *c, const k3cuda_token_batch *b) {
-    return PagedView{c->page_table, c->n_pages, c->page_size, c->max_pages,
-                     b->ctx_lens,   b->cu_tokens, b->B,       b->T};
+    int shift = 0;
+    while ((1 << shift) < c->page_size) shift++;
+    return PagedView{c->page_table, c->n_pages,   c->page_size, c->max_pages, b->ctx_lens,
+                     b->cu_tokens,  b->B,         b->T,         shift};
 }
 
 }  // namespace k3

@@ -13,23 +13,34 @@
 // one read of the cache serves all of them.
 //
 // The accumulator of o (128 x 512 fp32) takes all of an SM's TMEM, so a row tile is worked on by a
-// cluster of two CTAs with one job each. The score CTA holds the query in TMEM (288 columns, the A
-// operand), streams the tile's 576-wide rows, forms S and the softmax, and sends the weights P to
-// its peer as bf16 (asynchronous cluster stores that complete on an mbarrier), with the factor by
-// which o is to be rescaled. The value CTA streams the same rows' 512 latent dims, from L2 by then,
-// and accumulates o. P is double-buffered, so neither waits for the other in step.
-// What decides this split (measured on a B200): cluster stores move 17 B a clock and SM, TMA reads
-// from L2 over 70. Splitting the dims over the pair instead (each row read once, partial scores and
-// P exchanged, 36 KB per 96 rows and CTA) is bound by the former: 5400 cycles per 96 rows.
-// Tiles are 128 cache rows: an MMA takes about 60 cycles for any N up to 128 (60 at N = 64, 65.5 at
-// 128, 128.6 at 256, A in TMEM), so smaller tiles run the scores below the full rate.
+// cluster of two CTAs with one job each. The score CTA holds the query in TMEM (the A operand; its
+// rope dims in shared memory), streams the tile's 576-wide rows, forms S and the softmax, and sends
+// the weights P to its peer as bf16, with the factor by which o is to be rescaled. The value CTA
+// streams the same rows' 512 latent dims, from L2 by then, and accumulates o. S and P are
+// double-buffered, so neither CTA waits for the other in step.
+// What decides this layout (measured on a B200, cycles of an SM):
+//   * cluster stores move 17 B a clock and SM, TMA reads from L2 over 70. Splitting the dims over the
+//     pair instead (each row read once, partial scores and P exchanged, 36 KB per 96 rows and CTA)
+//     is bound by the former: 5400 cycles per 96 rows.
+//   * an MMA (M 128, A in TMEM) takes 74 cycles at N = 128 and 37 at N = 64, and the queue before the
+//     tensor core is a few MMAs deep: a wait of the issuing warp or a slow issue shows as idle tensor
+//     time. So tiles are 128 rows (N = 128: 64-row tiles took 5600 cycles per 128 rows), each chunk's
+//     barrier is looked at before the chunk before is fully issued, and P leaves by bulk copy (16-byte
+//     cluster stores from the softmax warps held up the MMAs behind them: +480 cycles per 64 rows).
+//   * a TMA instruction takes about 115 cycles to issue whatever it moves (4 KB boxes: 35 B a clock),
+//     so a chunk comes in one, through a four-dimensional view of the cache that lays eight-row
+//     groups [dim blocks][8 rows][128 B] one after another; pages of fewer rows take one each.
 // Per SM:
-//   score   TMEM: query 288 columns, S 128;  shared: 4 stages x 48 KB (three 64-dim blocks of 128
-//           rows, K-major, 128-byte swizzle)
-//   value   TMEM: o 512 columns;  shared: 4 stages x 32 KB (32 rows x 512 dims, MN-major), P 2 x 32 KB
-// Warps: 0 loads (a lane per box), 1 issues the MMAs, 2-17 are four groups of one warp per lane
-// quarter: in the score CTA a group takes 32 score columns of all rows, in the value CTA 128 dims
-// of o (rescaling, read-out).
+//   score   TMEM: query 256 columns, S 2 x 128;  shared: a tile in 4 stages of 32 KB (128 rows x 128
+//           dims, K-major), its rope dims 16 KB, the query's 16 KB, P 32 KB on its way out
+//   value   TMEM: o 512 columns;  shared: a tile in 4 stages of 32 KB (32 rows x 512 dims, MN-major),
+//           P 2 x 32 KB
+// Warps: 0 loads (a lane per page), 1 issues the MMAs, 2-9 are two groups of one warp per lane
+// quarter: in the score CTA a group takes 64 score columns of all rows, in the value CTA 256 dims
+// of o (rescaling, read-out). Warp 10 of the score CTA sends P, that of the value CTA brings rows into
+// L2. The warps share four schedulers, and
+// the score CTA's are busy half the time: sixteen softmax warps of 32 columns each slowed the loads
+// and the MMA issue by more than they gained.
 //
 // Work: the (row tile, cache tile) pairs lie on a line, every row tile taking TT_FIXED more places
 // for its fixed work; clusters take equal pieces (paged.cuh). A row tile that one cluster does
@@ -54,33 +65,43 @@ constexpr int TT_DN = 128, TT_DR = 64, TT_DL = 512, TT_DV = 128, TT_H = 128;
 constexpr int TT_QW = TT_DL + TT_DR;       // absorbed query width
 constexpr int TT_M = 128;                  // rows of a row tile
 constexpr int TT_TILE = 128;               // cache rows of a tile
-constexpr int TT_BOX = 32;                 // most rows of a load box
-constexpr int TT_NST = 4;                  // stages of either CTA
-constexpr int TT_KBLK = TT_TILE * 128;     // score: a 64-dim block of a tile; three to a stage
-constexpr int TT_KSTAGE = 3 * TT_KBLK;
-constexpr int TT_VROWS = 32;               // value: rows of a stage
-constexpr int TT_VBLK = TT_VROWS * 128;    // a 64-dim block of a value stage; eight to a stage
-constexpr int TT_VSTAGE = 8 * TT_VBLK;
-constexpr int TT_CHUNKS = TT_TILE / TT_VROWS;
-constexpr int TT_OFF_P = TT_NST * TT_VSTAGE;   // value: P, two buffers of two 64-column blocks
-constexpr int TT_PBUF = 2 * TT_M * 128;
-constexpr int TT_SMEM = TT_NST * TT_KSTAGE + 1024;
-static_assert(TT_CHUNKS == TT_NST, "chunk c of every tile is in stage c");
-static_assert(TT_OFF_P + 2 * TT_PBUF <= TT_SMEM - 1024, "both CTAs' layouts fit");
-constexpr int TT_TM_Q = 0, TT_TM_S = 288, TT_TM_COLS = 512;
-constexpr int TT_CW = TT_TILE / 4;         // score columns of a softmax warp
-constexpr int TT_WORKERS = 16;             // warps 2 .. 17
-constexpr int TT_THREADS = (2 + TT_WORKERS) * 32;
+constexpr int TT_KCH = 4, TT_VCH = 4;      // chunks of a tile, one to a stage: by dims, by rows
+constexpr int TT_KSTAGE = TT_TILE * TT_DL * 2 / TT_KCH;
+constexpr int TT_VROWS = TT_TILE / TT_VCH;
+constexpr int TT_VSTAGE = TT_VROWS * TT_DL * 2;
+constexpr int TT_AHEAD = 4;                // tiles that rows are brought into L2 before their load
+constexpr int TT_PBUF = 2 * TT_M * 128;    // two blocks of 64 columns
+constexpr int TT_OFF_KR = TT_KCH * TT_KSTAGE;     // score: rope dims of the tile
+constexpr int TT_OFF_QR = TT_OFF_KR + TT_TILE * 128;  // and of the query
+constexpr int TT_OFF_PS = TT_OFF_QR + TT_M * 128;     // P on its way out
+constexpr int TT_OFF_FS = TT_OFF_PS + TT_PBUF;        // its rescale factors
+constexpr int TT_GRP = 2;                  // groups of worker warps, one warp per lane quarter each
+constexpr int TT_OFF_VAL = TT_OFF_FS + TT_M * 4;      // values shared by a row's warps
+constexpr int TT_OFF_P = TT_VCH * TT_VSTAGE;      // value: P, two buffers
+constexpr int TT_OFF_F = TT_OFF_P + 2 * TT_PBUF;  // and their factors
+constexpr int TT_SMEM = TT_OFF_VAL + 2 * TT_GRP * TT_M * 4 + 1024;
+static_assert(TT_OFF_F + 2 * TT_M * 4 <= TT_SMEM - 1024, "both CTAs' layouts fit");
+constexpr int TT_TM_Q = 0, TT_TM_S = 256, TT_TM_COLS = 512;
+constexpr int TT_CW = TT_TILE / TT_GRP;    // score columns of a softmax warp
+constexpr int TT_OW = TT_DL / TT_GRP;      // dims of o of a warp in the value CTA
+constexpr int TT_WORKERS = 4 * TT_GRP;     // warps 2 ..
+constexpr int TT_THREADS = (3 + TT_WORKERS) * 32;
 constexpr int TT_CLUSTERS = 74;            // 148 SMs of a B200
 constexpr int TT_FIXED = 4;                // a row tile's fixed work, in tiles
 constexpr int TT_MIN_TILES = 2;            // fewest tiles per cluster
 constexpr int TT_PART = TT_DL + 4;         // floats of a partial row: o, m, l, pad
-constexpr uint32_t TT_P_BYTES = TT_PBUF + TT_M * 4;  // P and the rescale factors of a tile
+// A row tile that is cut and begins in some cluster: the last cluster with a part of it (-1: the
+// cluster begins none), its rows, and its first row among all (token, head) rows.
+struct TreeCut {
+    int last, rows;
+    long long row0;
+};
 
 // the device-side plan, at the start of the workspace
 struct TreePlan {
     long long total;   // places on the line
     int G;             // clusters that take part
+    TreeCut cut[TT_CLUSTERS];
 };
 
 struct TreeArgs {
@@ -88,6 +109,7 @@ struct TreeArgs {
     const TreePlan *plan;
     const long long *cum;      // [B + 1] first place of each sequence
     const unsigned long long *mask;
+    const __nv_bfloat16 *latent, *rope;  // the cache's rows
     const __nv_bfloat16 *qlat; // [T][H][576]
     float *part;               // [2 TT_CLUSTERS][128][TT_PART]
     __nv_bfloat16 *olat2;      // [T][H][hi 512 | lo 512]
@@ -98,7 +120,7 @@ struct TreeArgs {
 };
 
 struct TreeMaps {
-    CUtensorMap lat, rope;
+    CUtensorMap lat_k, lat_v, rope;
 };
 
 // A cluster's next piece of the line: tiles t0 .. t1 - 1 of row tile mt of sequence b.
@@ -204,29 +226,41 @@ __global__ void __launch_bounds__(1024) mla_tree_plan(PagedView v, int H, TreePl
         plan->total = carry;
         plan->G = (int)(want < clusters ? want : clusters);
     }
-}
-
-// A bounded wait taken by one lane for its warp: 32 lanes that poll one barrier take the
-// shared-memory pipe from everybody else.
-template <bool kCluster = false>
-__device__ __forceinline__ bool lane_wait(uint64_t *bar, uint32_t parity, unsigned *err,
-                                          unsigned code) {
-    bool ok = true;
-    if ((threadIdx.x & 31) == 0) ok = mbar_wait_impl<kCluster>(bar, parity, err, code);
-    __syncwarp();  // what lane 0 has seen, every lane sees
-    return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+    __syncthreads();
+    // the row tile that holds each cluster's last place
+    const int G = plan->G;
+    const long long total = carry;
+    if (tid < TT_CLUSTERS) {
+        TreeCut cut{-1, 0, 0};
+        if (tid + 1 < G) {
+            const long long end = line_begin(total, G, tid + 1);
+            const int b = last_at_most(cum, v.B, end - 1);
+            const PagedSeq s = paged_seq(v, b, K3CUDA_MAX_DRAFTS);
+            const long long cost = TT_FIXED + (s.len + s.n + TT_TILE - 1) / TT_TILE;
+            const int mt = (int)((end - 1 - cum[b]) / cost);
+            const long long first = cum[b] + mt * cost + TT_FIXED, last = first + cost - TT_FIXED - 1;
+            // some of its tiles are in this cluster, the first among them, and some are not
+            if (first < end && end <= last && first >= line_begin(total, G, tid)) {
+                cut.last = line_cluster(total, G, last);
+                cut.rows = min(TT_M, s.n * H - mt * TT_M);
+                cut.row0 = (long long)s.first * H + mt * TT_M;
+            }
+        }
+        plan->cut[tid] = cut;
+    }
 }
 
 struct TreeBars {
-    uint64_t full[TT_NST], empty[TT_NST];  // stages
-    uint64_t q_full, q_empty, s_full, s_empty;  // score
-    uint64_t pair[4];           // score: per lane quarter, its four warps
-    uint64_t p_in[2], p_full[2];  // value: P has come; o is ready for it
-    uint64_t pv_done[2];        // both: o of the tile is done, P's buffer free
-    uint64_t clean[TT_CHUNKS];  // value: the stages of a tile that reaches past the cached rows
-    float val[2][4][TT_M];      // score: row maxima (or sums) of the four warps, by phase parity
-    float fac[2][TT_M];         // value: rescale factors
+    uint64_t full[TT_KCH], empty[TT_KCH];  // stages
+    uint64_t q_full, q_empty;              // score: queries in place; their last S is done
+    uint64_t s_full[2], s_empty[2];        // score
+    uint64_t pair[4];                      // score: per lane quarter, its two warps
+    uint64_t p_out, p_ack;                 // score: P is written; the peer has it
+    uint64_t p_in[2], p_full[2];           // value: P has come; o is ready for it
+    uint64_t pv_done[2];                   // both: o of the tile is done, P's buffer free
+    uint64_t clean[TT_VCH];                // value: stages that reach past the cached rows
     uint32_t tmem_base;
+    int tile;                              // value: the tile being loaded
 };
 
 // n columns of o from addr: multiply by f
@@ -275,18 +309,23 @@ __device__ __forceinline__ void write_o(const TreeArgs &a, const TreeSeg &g, int
     }
 }
 
-// A row tile's queries into TMEM (lane = row, two bf16 per column): group grp of a quarter takes
-// every fourth 64-dim block. Rows past the last token's are zero.
+// A row tile's queries: the latent dims into TMEM (lane = row, two bf16 per column), group grp of a
+// quarter one half of them; the rope dims into shared memory, 32 dims a group. Rows past the last
+// token's are zero.
 __device__ __forceinline__ void load_q(const TreeArgs &a, const TreeSeg &g, uint32_t lane_addr,
-                                       int row, int grp) {
+                                       uint8_t *rope, int row, int grp) {
     const int lr = g.mt * TT_M + row;
     const bool ok = lr < g.s.n * a.H;
     const uint4 *q = reinterpret_cast<const uint4 *>(a.qlat + ((size_t)g.s.first * a.H + lr) * TT_QW);
-    for (int h = 2 * grp; h < 18; h += h & 1 ? 7 : 1) {  // half blocks: 32 dims, 16 columns
+    const uint4 none = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 4 * grp; i < 4 * grp + 4; i++)
+        st16s(rope + swz(row, i), ok ? q[TT_DL / 8 + i] : none);
+    for (int h = 8 * grp; h < 8 * grp + 8; h++) {  // half blocks: 32 dims, 16 columns
         float v[16];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const uint4 w = ok ? q[4 * h + i] : make_uint4(0, 0, 0, 0);
+            const uint4 w = ok ? q[4 * h + i] : none;
             v[4 * i] = __uint_as_float(w.x);
             v[4 * i + 1] = __uint_as_float(w.y);
             v[4 * i + 2] = __uint_as_float(w.z);
@@ -297,17 +336,6 @@ __device__ __forceinline__ void load_q(const TreeArgs &a, const TreeSeg &g, uint
     tmem_wait_st();
 }
 
-// The rows of a tile's load boxes: box j holds rows j box .. of the tile.
-__device__ __forceinline__ int box_row(const TreeArgs &a, const TreeSeg &g, long long pos,
-                                       bool report) {
-    long long r = paged_row(a.v, g.b, (int)pos);
-    if (r < 0) {
-        if (report) atomicCAS(a.err + 1, 0u, (unsigned)PAGED_PAGE);
-        r = pos % a.v.page_size;
-    }
-    return (int)r;
-}
-
 // Zero what a draft row of bf16 pairs holds that is not finite.
 __device__ __forceinline__ uint32_t finite_pair(uint32_t u) {
     if ((u & 0x7f80u) == 0x7f80u) u &= 0xffff0000u;
@@ -315,77 +343,129 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t u) {
     return u;
 }
 
-// ---------------------------------------------------------------- score CTA
-__device__ __forceinline__ void score_loads(const TreeMaps &maps, const TreeArgs &a, TreeWalk walk,
-                                            uint8_t *sm, TreeBars &bars) {
+// A CTA's loads, chunk by chunk: for the score CTA 128 rows x 128 latent dims, the rope dims with
+// the first; for the value CTA 64 rows x 512 dims. Chunk c of every tile is in stage c.
+template <bool kScore>
+__device__ __forceinline__ void tree_loads(const TreeMaps &maps, const TreeArgs &a, TreeWalk walk,
+                                           uint8_t *sm, TreeBars &bars) {
+    constexpr int CH = kScore ? TT_KCH : TT_VCH, ROWS = kScore ? TT_TILE : TT_VROWS;
+    constexpr int STAGE = kScore ? TT_KSTAGE : TT_VSTAGE, RB = STAGE / ROWS;  // bytes of a row
     const int lane = threadIdx.x & 31;
-    const int box = a.v.page_size < TT_BOX ? a.v.page_size : TT_BOX, boxes = TT_TILE / box;
-    int i = 0;  // stages filled
-    bool ok = true;
+    const int box = min(a.v.page_size, ROWS), per = ROWS / box;  // rows of a box, boxes of a chunk
+    int g = 0, loaded = 0;  // tiles; stages in use
+    // this lane's box of a tile: its first cache row (page 0 where the table names no page)
+    auto lookup = [&](const TreeSeg &sg, int t) -> int {
+        const int p = t * TT_TILE + lane * box;
+        if (lane >= TT_TILE / box || p >= sg.s.len + sg.s.n) return 0;
+        long long r = paged_row(a.v, sg.b, p);
+        if (r < 0) {
+            if (kScore) atomicCAS(a.err + 1, 0u, (unsigned)PAGED_PAGE);
+            r = p & (a.v.page_size - 1);
+        }
+        return (int)r;
+    };
     TreeSeg sg;
-    while (ok && walk.next(sg)) {
-        for (int t = sg.t0; t < sg.t1 && ok; t++) {
-            const long long p0 = (long long)t * TT_TILE;
-            const int rows = sg.s.len + sg.s.n;
-            const int live = (int)min((long long)boxes, (rows - p0 + box - 1) / box);
-            // a lane's boxes are the same in each of the tile's three stages (boxes <= 16, three
-            // blocks: up to two loads a lane)
-            int row[2];
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const int j = (lane + 32 * k) % boxes;
-                row[k] = 0;
-                if (lane + 32 * k < 3 * boxes && j < live)
-                    row[k] = box_row(a, sg, p0 + j * box, true);
+    bool more = walk.next(sg), ok = true;
+    int t = more ? sg.t0 : 0, row = more ? lookup(sg, t) : 0;
+    for (; more && ok; g++) {
+        const int live = (sg.s.len + sg.s.n - t * TT_TILE + box - 1) / box, at = row;
+        if (!kScore && lane == 0) *(volatile int *)&bars.tile = g;
+        // the next tile's rows, looked up under this one's loads
+        if (++t >= sg.t1) {
+            more = walk.next(sg);
+            t = more ? sg.t0 : 0;
+        }
+        if (more) row = lookup(sg, t);
+#pragma unroll 1
+        for (int c = 0; c < CH; c++) {
+            // the lanes whose boxes this chunk takes: all of them, or those of its rows
+            const int first = kScore ? 0 : c * per, j = lane - first;
+            const int n = max(0, min(per, live - first));
+            const bool rope = kScore && c == 0;
+            if (g > 0 && !(ok = warp_spin(&bars.empty[c], (g - 1) & 1, a.err, 0x501))) break;
+            if (lane == 0) mbar_expect_tx(&bars.full[c], n * box * (RB + (rope ? 128 : 0)));
+            __syncwarp();
+            if (j >= 0 && j < n) {
+                tma_load_4d(sm + c * STAGE + j * box * RB, kScore ? &maps.lat_k : &maps.lat_v,
+                            &bars.full[c], 0, 0, kScore ? c * (RB / 128) : 0, at / 8);
+                if (rope)
+                    tma_load_2d(sm + TT_OFF_KR + j * box * 128, &maps.rope, &bars.full[c], 0, at);
             }
-            for (int c = 0; c < 3; c++, i++) {
-                const int st = i % TT_NST, n = i / TT_NST;
-                if (n > 0 && !(ok = lane_wait(&bars.empty[st], (n - 1) & 1, a.err, 0x502))) break;
-                if (lane == 0) mbar_expect_tx(&bars.full[st], live * box * 3 * 128);
-                __syncwarp();
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const int e = lane + 32 * k, j = e % boxes, kb = 3 * c + e / boxes;
-                    if (e >= 3 * boxes || j >= live) continue;
-                    uint8_t *dst = sm + st * TT_KSTAGE + (e / boxes) * TT_KBLK + j * box * 128;
-                    if (kb < 8) tma_load_2d(dst, &maps.lat, &bars.full[st], kb * 64, row[k]);
-                    else tma_load_2d(dst, &maps.rope, &bars.full[st], 0, row[k]);
-                }
-            }
+            loaded = (loaded & ~(3 << (2 * c))) | ((g & 1 ? 2 : 1) << (2 * c));
         }
     }
     // loads still in flight are waited for (bounded) before the CTA may exit
     if (lane == 0)
-        for (int st = 0; st < TT_NST && st < i; st++)
-            mbar_wait_quiet(&bars.full[st], ((i - 1 - st) / TT_NST) & 1);
+        for (int c = 0; c < CH; c++)
+            if ((loaded >> (2 * c)) & 3) mbar_wait_quiet(&bars.full[c], (loaded >> (2 * c)) & 2 ? 1 : 0);
     __syncwarp();
+}
+
+// ---------------------------------------------------------------- score CTA
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t &>(d))
+        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)),
+          "l"(reinterpret_cast<uint64_t &>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t &>(d))
+        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return d;
 }
 
 __device__ __forceinline__ void score_mma(const TreeArgs &a, TreeWalk walk, uint8_t *sm,
                                           TreeBars &bars, uint32_t tbase) {
     constexpr uint32_t id = idesc_f16(128, TT_TILE, false, false);
-    int g = 0, i = 0, nq = 0;
+    int g = 0, nq = 0;
+    bool data = false, room = true;  // the next chunk and score buffer, as seen in advance
     TreeSeg sg;
     while (walk.next(sg)) {
-        if (!mbar_wait(&bars.q_full, nq++ & 1, a.err, 0x511)) return;
+        if (!warp_spin(&bars.q_full, nq++ & 1, a.err, 0x511)) return;
         for (int t = sg.t0; t < sg.t1; t++, g++) {
-            for (int c = 0; c < 3; c++, i++) {
-                const int st = i % TT_NST;
-                if (!mbar_wait(&bars.full[st], (i / TT_NST) & 1, a.err, 0x512)) return;
-                if (c == 0 && g >= 1 && !mbar_wait(&bars.s_empty, (g - 1) & 1, a.err, 0x513)) return;
+            const int sb = g & 1;
+            const uint32_t d = tbase + TT_TM_S + sb * TT_TILE;
+            uint32_t q = tbase + TT_TM_Q;
+            if (!room && !warp_spin(&bars.s_empty[sb], ((g >> 1) - 1) & 1, a.err, 0x512)) return;
+#pragma unroll 1
+            for (int c = 0; c < TT_KCH; c++) {
+                if (!data && !warp_spin(&bars.full[c], g & 1, a.err, 0x513)) return;
                 tc_fence_after();
-                const uint32_t kv = smem_u32(sm + st * TT_KSTAGE);
-#pragma unroll
-                for (int kb = 0; kb < 3; kb++)
+                uint64_t b = sdesc(smem_u32(sm + c * TT_KSTAGE), 16, 2048);
+                if (c == 0) {
+                    const uint64_t qr = sdesc_kmajor(smem_u32(sm + TT_OFF_QR));
+                    const uint64_t kr = sdesc_kmajor(smem_u32(sm + TT_OFF_KR));
 #pragma unroll
                     for (int ks = 0; ks < 4; ks++)
-                        mma_bf16_ts(tbase + TT_TM_S, tbase + TT_TM_Q + (3 * c + kb) * 32 + ks * 8,
-                                    sdesc_kmajor(kv + kb * TT_KBLK + ks * 32), id,
-                                    (c | kb | ks) ? 1u : 0u);
-                mma_commit(&bars.empty[st]);
+                        warp_mma_ss(d, qr + ks * (32 >> 4), kr + ks * (32 >> 4), id, ks ? 1u : 0u);
+                }
+#pragma unroll
+                for (int ks = 0; ks < 4; ks++) warp_mma_ts(d, q + ks * 8, b + ks * (32 >> 4), id, 1u);
+                if (c + 1 < TT_KCH) {
+                    data = __all_sync(0xffffffffu, mbar_test(&bars.full[c + 1], g & 1));
+                } else {
+                    data = __all_sync(0xffffffffu, mbar_test(&bars.full[0], (g + 1) & 1));
+                    room = g < 1 || __all_sync(0xffffffffu, mbar_test(&bars.s_empty[sb ^ 1],
+                                                                          (((g + 1) >> 1) - 1) & 1));
+                }
+                q += 32;
+                b += 1024 >> 4;
+#pragma unroll
+                for (int ks = 0; ks < 4; ks++) warp_mma_ts(d, q + ks * 8, b + ks * (32 >> 4), id, 1u);
+                q += 32;
+                if (c + 1 == TT_KCH) warp_commit(&bars.s_full[sb]);
+                warp_commit(&bars.empty[c]);
             }
-            mma_commit(&bars.s_full);
-            if (t + 1 == sg.t1) mma_commit(&bars.q_empty);
+            if (t + 1 == sg.t1) warp_commit(&bars.q_empty);
         }
     }
 }
@@ -397,28 +477,32 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
     const int row = 32 * q4 + lane;                  // row of the row tile = TMEM lane
     const int c0 = TT_CW * grp;                      // first score column
     const uint32_t laddr = tbase + ((uint32_t)(32 * q4) << 16);
-    const uint32_t ppeer = map_peer(smem_u32(sm + TT_OFF_P), 1);
-    const uint32_t fpeer = map_peer(smem_u32(&bars.fac[0][row]), 1);
-    const uint32_t bpeer = map_peer(smem_u32(&bars.p_in[0]), 1);
+    uint8_t *P = sm + TT_OFF_PS + grp * (TT_M * 128);  // this warp's 64-column block
+    float *val = reinterpret_cast<float *>(sm + TT_OFF_VAL) + row;  // [2][TT_GRP][TT_M]
+    // Scores are scaled to log2 units with the maximum's subtraction, by a positive factor (a masked
+    // -inf stays one): a negative scale changes their sign first, a scale of zero makes them zero.
+    const float scale = a.scale_log2e == 0.f ? 1.f : fabsf(a.scale_log2e);
+    const float sign = a.scale_log2e > 0.f ? 1.f : a.scale_log2e < 0.f ? -1.f : 0.f;
     float m_ref = -INFINITY, l = 0.f;  // l: this warp's columns
     int g = 0, nq = 0, np = 0;
-    // the row's values of the quarter's four warps
-    auto share = [&](float v, float (&o)[4]) -> bool {
-        bars.val[np & 1][grp][row] = v;
+    // the other warp's value of the row
+    auto share = [&](float v, float &o) -> bool {
+        float *at = val + (np & 1) * TT_GRP * TT_M;
+        at[grp * TT_M] = v;
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.pair[q4]);
-        if (!lane_wait(&bars.pair[q4], np & 1, a.err, 0x521)) return false;
-#pragma unroll
-        for (int i = 0; i < 4; i++) o[i] = bars.val[np & 1][i][row];
+        if (!warp_spin(&bars.pair[q4], np & 1, a.err, 0x521)) return false;
+        o = at[(grp ^ 1) * TT_M];
         np++;
         return true;
     };
     TreeSeg sg;
     while (walk.next(sg)) {
         // this warp's part of the queries (the last row tile's S must be done)
-        if (nq > 0 && !lane_wait(&bars.q_empty, (nq - 1) & 1, a.err, 0x522)) return;
+        if (nq > 0 && !warp_spin(&bars.q_empty, (nq - 1) & 1, a.err, 0x522)) return;
         tc_fence_after();
-        load_q(a, sg, laddr, row, grp);
+        load_q(a, sg, laddr, sm + TT_OFF_QR, row, grp);
+        fence_async_shared();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.q_full);
@@ -427,34 +511,38 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
         const int tok = min((sg.mt * TT_M + row) / a.H, sg.s.n - 1);
         const uint64_t word = a.mask ? a.mask[sg.s.first + tok] : (((uint64_t)2 << tok) - 1);
         for (int t = sg.t0; t < sg.t1; t++, g++) {
+            const int sb = g & 1;
             float s[TT_CW];
-            if (!lane_wait(&bars.s_full, g & 1, a.err, 0x523)) return;
+            if (!warp_spin(&bars.s_full[sb], (g >> 1) & 1, a.err, 0x523)) return;
             tc_fence_after();
-            tmem_ld32(laddr + TT_TM_S + c0, s);
+            tmem_ld32(laddr + TT_TM_S + sb * TT_TILE + c0, s);
+            tmem_ld32(laddr + TT_TM_S + sb * TT_TILE + c0 + 32, s + 32);
             tmem_wait_ld();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.s_empty);
-            const long long p0 = (long long)t * TT_TILE + c0;
+            if (lane == 0) mbar_arrive(&bars.s_empty[sb]);
+            if (sign != 1.f) {
+#pragma unroll
+                for (int i = 0; i < TT_CW; i++) s[i] *= sign;
+            }
+            const int p0 = t * TT_TILE + c0;
             if (p0 + TT_CW > sg.s.len) {  // reaches past the cached rows
-                const uint32_t see = (uint32_t)tree_bits(word, sg.s.len, sg.s.n, p0);
-                const int d0 = (int)max(0ll, min((long long)TT_CW, sg.s.len - p0));
+                const uint64_t see = tree_bits(word, sg.s.len, sg.s.n, p0);
+                const int d0 = sg.s.len - p0;
 #pragma unroll
                 for (int i = 0; i < TT_CW; i++) {
                     if (i >= d0 && !(fabsf(s[i]) < INFINITY)) s[i] = NAN;
-                    // (a negative scale would turn the mask into +inf)
-                    s[i] = (see >> i) & 1 ? s[i] * a.scale_log2e : -INFINITY;
+                    if (!((see >> i) & 1)) s[i] = -INFINITY;
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < TT_CW; i++) s[i] *= a.scale_log2e;
             }
             float m4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int i = 4; i < TT_CW; i++) m4[i & 3] = fmaxf(m4[i & 3], s[i]);
-            float o[4];
-            if (!share(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), o)) return;
-            const float mx = fmaxf(fmaxf(o[0], o[1]), fmaxf(o[2], o[3]));
+            for (int i = 4; i < TT_CW; i += 8)
+#pragma unroll
+                for (int j = 0; j < 4; j++) m4[j] = max3(m4[j], s[i + j], i + 4 < TT_CW ? s[i + 4 + j] : s[i + j]);
+            float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale, o;
+            if (!share(mx, o)) return;
+            mx = fmaxf(mx, o);
             float f = 1.f;
             if (t == sg.t0) {
                 m_ref = mx;
@@ -466,33 +554,35 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
             }
             const float base = m_ref == -INFINITY ? 0.f : m_ref;  // nothing seen so far
             uint32_t w[TT_CW / 2];
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const float2 k2 = make_float2(scale, scale), b2 = make_float2(-base, -base);
+            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
             for (int i = 0; i < TT_CW; i += 2) {
-                const float a0 = ex2_approx(s[i] - base), a1 = ex2_approx(s[i + 1] - base);
-                sum[(i >> 1) & 3] += a0 + a1;
-                w[i / 2] = pack_bf2(a0, a1);
+                float2 e = fma2(make_float2(s[i], s[i + 1]), k2, b2);
+                e.x = ex2_approx(e.x);
+                e.y = ex2_approx(e.y);
+                sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
+                w[i / 2] = pack_bf2(e.x, e.y);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            // P to the peer: 16-byte chunk ch of a row, 64 columns to a block, swizzled
-            const int pb = g & 1;
-            if (g >= 2 && !lane_wait(&bars.pv_done[pb], ((g >> 1) - 1) & 1, a.err, 0x524)) return;
-            const uint32_t rbar = bpeer + 8 * pb;
+            sum[0] = add2(sum[0], sum[1]);
+            l += sum[0].x + sum[0].y;
+            // P as the MMA will read it: 16-byte chunk ch of a row of 64 columns, swizzled
+            if (g >= 1 && !warp_spin<true>(&bars.p_ack, (g - 1) & 1, a.err, 0x524)) return;
 #pragma unroll
-            for (int c = 0; c < TT_CW / 8; c++) {
-                const int ch = c0 / 8 + c;
-                st_async_v4(ppeer + pb * TT_PBUF + (ch >> 3) * (TT_M * 128) + swz(row, ch & 7),
-                            __uint_as_float(w[4 * c]), __uint_as_float(w[4 * c + 1]),
-                            __uint_as_float(w[4 * c + 2]), __uint_as_float(w[4 * c + 3]), rbar);
-            }
-            if (grp == 0) st_async_f32(fpeer + pb * TT_M * 4, f, rbar);
+            for (int c = 0; c < TT_CW / 8; c++)
+                st16s(P + swz(row, c),
+                      make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
+            if (grp == 0) reinterpret_cast<float *>(sm + TT_OFF_FS)[row] = f;
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.p_out);
         }
         // the row's sum
-        float o[4];
+        float o;
         if (!share(l, o)) return;
         const int lr = sg.mt * TT_M + row;
         if (grp == 0 && lr < sg.s.n * a.H) {
-            const float lt = (o[0] + o[1]) + (o[2] + o[3]);
+            const float lt = l + o;
             if (sg.whole()) a.rowsum[(size_t)sg.s.first * a.H + lr] = lt;
             else {
                 float *dst = a.part + ((size_t)sg.slot(cl) * TT_M + row) * TT_PART + TT_DL;
@@ -501,76 +591,102 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
             }
         }
     }
-    // the peer is done with every P (its last commits arrive on this CTA's barriers)
-    for (int k = g >= 2 ? g - 2 : 0; k < g; k++)
-        if (!lane_wait(&bars.pv_done[k & 1], (k >> 1) & 1, a.err, 0x525)) return;
 }
 
-// ---------------------------------------------------------------- value CTA
-__device__ __forceinline__ void value_loads(const TreeMaps &maps, const TreeArgs &a, TreeWalk walk,
-                                            uint8_t *sm, TreeBars &bars) {
-    const int lane = threadIdx.x & 31;
-    const int box = a.v.page_size < TT_BOX ? a.v.page_size : TT_BOX, boxes = TT_VROWS / box;
-    int i = 0;
-    bool ok = true;
-    TreeSeg sg;
-    while (ok && walk.next(sg)) {
-        for (int t = sg.t0; t < sg.t1 && ok; t++) {
-            const long long rows = sg.s.len + sg.s.n;
-            for (int c = 0; c < TT_CHUNKS; c++, i++) {
-                const int st = i % TT_NST, n = i / TT_NST;
-                // lane: box lane % boxes of 64-dim block lane / boxes
-                const int j = lane % boxes, kb = lane / boxes;
-                const long long p0 = (long long)t * TT_TILE + c * TT_VROWS;
-                const int live =
-                    (int)max(0ll, min((long long)boxes, (rows - p0 + box - 1) / box));
-                const bool some = j < live && kb < 8;
-                const int row = some ? box_row(a, sg, p0 + j * box, false) : 0;
-                if (n > 0 && !(ok = lane_wait(&bars.empty[st], (n - 1) & 1, a.err, 0x532))) break;
-                if (lane == 0) mbar_expect_tx(&bars.full[st], live * box * 8 * 128);
-                __syncwarp();
-                if (some)
-                    tma_load_2d(sm + st * TT_VSTAGE + kb * TT_VBLK + j * box * 128, &maps.lat,
-                                &bars.full[st], kb * 64, row);
-            }
-        }
-    }
-    if (lane == 0)
-        for (int st = 0; st < TT_NST && st < i; st++)
-            mbar_wait_quiet(&bars.full[st], ((i - 1 - st) / TT_NST) & 1);
-    __syncwarp();
-}
-
-__device__ __forceinline__ void value_mma(const TreeArgs &a, TreeWalk walk, uint8_t *sm,
-                                          TreeBars &bars, uint32_t tbase) {
-    constexpr uint32_t id = idesc_f16(128, 256, false, true);
-    int g = 0, i = 0, edges = 0;
+// P to the peer as soon as it is written and the buffer there is free.
+__device__ __forceinline__ void score_send(const TreeArgs &a, TreeWalk walk, uint8_t *sm,
+                                           TreeBars &bars) {
+    const uint32_t ps = smem_u32(sm + TT_OFF_PS), fs = smem_u32(sm + TT_OFF_FS);
+    const uint32_t pd = map_peer(smem_u32(sm + TT_OFF_P), 1), fd = map_peer(smem_u32(sm + TT_OFF_F), 1);
+    const uint32_t bar = map_peer(smem_u32(&bars.p_in[0]), 1);
+    const bool lead = (threadIdx.x & 31) == 0;
+    int g = 0;
     TreeSeg sg;
     while (walk.next(sg)) {
         for (int t = sg.t0; t < sg.t1; t++, g++) {
-            if (!mbar_wait(&bars.p_full[g & 1], (g >> 1) & 1, a.err, 0x541)) return;
-            const bool edge = (long long)(t + 1) * TT_TILE > sg.s.len;
-            const uint32_t P = smem_u32(sm + TT_OFF_P + (g & 1) * TT_PBUF);
-            for (int c = 0; c < TT_CHUNKS; c++, i++) {
-                const int st = i % TT_NST;
-                if (!mbar_wait(&bars.full[st], (i / TT_NST) & 1, a.err, 0x542)) return;
-                if (edge && !mbar_wait(&bars.clean[c], edges & 1, a.err, 0x543)) return;
-                tc_fence_after();
-                const uint32_t kv = smem_u32(sm + st * TT_VSTAGE);
-#pragma unroll
-                for (int ks = 0; ks < TT_VROWS / 16; ks++) {
-                    const int k = c * (TT_VROWS / 16) + ks;  // 16 rows of the tile
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        mma_bf16_ss(tbase + 256 * h,
-                                    sdesc_kmajor(P + (k >> 2) * (TT_M * 128) + (k & 3) * 32),
-                                    sdesc_mnmajor(kv + h * 4 * TT_VBLK + ks * 2048, TT_VBLK), id,
-                                    (t == sg.t0 && k == 0) ? 0u : 1u);
-                }
-                mma_commit(&bars.empty[st]);
+            const int pb = g & 1;
+            if (!warp_spin(&bars.p_out, g & 1, a.err, 0x531)) return;
+            if (g >= 2 && !warp_spin(&bars.pv_done[pb], ((g >> 1) - 1) & 1, a.err, 0x532)) return;
+            if (lead) {
+                bulk_send(pd + pb * TT_PBUF, ps, TT_PBUF, bar + 8 * pb);
+                bulk_send(fd + pb * TT_M * 4, fs, TT_M * 4, bar + 8 * pb);
             }
-            mma_commit_cluster(&bars.pv_done[g & 1], 3);
+            __syncwarp();
+        }
+    }
+    // the peer's last arrivals on this CTA's barriers
+    if (g > 0 && !warp_spin<true>(&bars.p_ack, (g - 1) & 1, a.err, 0x533)) return;
+    for (int k = g >= 2 ? g - 2 : 0; k < g; k++)
+        if (!warp_spin(&bars.pv_done[k & 1], (k >> 1) & 1, a.err, 0x534)) return;
+}
+
+// ---------------------------------------------------------------- value CTA
+__device__ __forceinline__ void value_mma(const TreeArgs &a, TreeWalk walk, uint8_t *sm,
+                                          TreeBars &bars, uint32_t tbase) {
+    constexpr uint32_t id = idesc_f16(128, 256, false, true);
+    int g = 0, edges = 0;
+    bool data = false, ready = false;  // the next chunk and P, as seen in advance
+    TreeSeg sg;
+    while (walk.next(sg)) {
+        for (int t = sg.t0; t < sg.t1; t++, g++) {
+            const int pb = g & 1;
+            const bool edge = (long long)(t + 1) * TT_TILE > sg.s.len;
+            if (!ready && !warp_spin(&bars.p_full[pb], (g >> 1) & 1, a.err, 0x541)) return;
+#pragma unroll 1
+            for (int c = 0; c < TT_VCH; c++) {
+                if (!data && !warp_spin(&bars.full[c], g & 1, a.err, 0x542)) return;
+                if (edge && !warp_spin(&bars.clean[c], edges & 1, a.err, 0x543)) return;
+                tc_fence_after();
+                // 16 rows at a time: P's columns, the rows' 512 dims in two halves
+                const uint64_t kv = sdesc(smem_u32(sm + c * TT_VSTAGE), 1024, 8192);
+                const uint64_t pd = sdesc_kmajor(
+                    smem_u32(sm + TT_OFF_P + pb * TT_PBUF + (c >> 1) * TT_M * 128 + (c & 1) * 64));
+                const uint32_t acc = (t == sg.t0 && c == 0) ? 0u : 1u;
+                warp_mma_ss(tbase, pd, kv, id, acc);
+                warp_mma_ss(tbase + 256, pd, kv + (4096 >> 4), id, acc);
+                warp_mma_ss(tbase, pd + (32 >> 4), kv + (16384 >> 4), id, 1u);
+                if (c + 1 < TT_VCH) {
+                    data = __all_sync(0xffffffffu, mbar_test(&bars.full[c + 1], g & 1));
+                } else {
+                    data = __all_sync(0xffffffffu, mbar_test(&bars.full[0], (g + 1) & 1));
+                    ready = __all_sync(0xffffffffu,
+                                       mbar_test(&bars.p_full[pb ^ 1], ((g + 1) >> 1) & 1));
+                }
+                warp_mma_ss(tbase + 256, pd + (32 >> 4), kv + (20480 >> 4), id, 1u);
+                if (c + 1 == TT_VCH) warp_commit_cluster(&bars.pv_done[pb], 3);
+                warp_commit(&bars.empty[c]);
+            }
             edges += edge;
+        }
+    }
+}
+
+// Bring the rows of the tiles to come into L2 (both CTAs' loads find them there): the score CTA's
+// stages do not cover the latency of HBM under load, about 3000 cycles. Plain prefetches: TMA's take
+// as much of its time as the loads. The score CTA's loads run two to three tiles before this CTA's.
+__device__ __forceinline__ void value_prefetch(const TreeArgs &a, TreeWalk walk, TreeBars &bars) {
+    const int lane = threadIdx.x & 31, box = min(a.v.page_size, TT_TILE);
+    const long long t0 = clock64();
+    int g = 0;
+    TreeSeg sg;
+    while (walk.next(sg)) {
+        for (int t = sg.t0; t < sg.t1; t++, g++) {
+            while (g > *(volatile int *)&bars.tile + TT_AHEAD) {
+                __nanosleep(400);
+                if (*(volatile unsigned *)a.err || clock64() - t0 > wait_limit(a.err)) return;
+            }
+            const int end = min((t + 1) * TT_TILE, sg.s.len + sg.s.n);
+            for (int p = t * TT_TILE; p < end; p += box) {
+                const long long row = paged_row(a.v, sg.b, p);
+                if (row < 0) continue;
+                const int rows = min(box, end - p);
+                const char *lat = reinterpret_cast<const char *>(a.latent + row * TT_DL);
+                const char *rope = reinterpret_cast<const char *>(a.rope + row * TT_DR);
+                for (int e = lane; e < rows * 8; e += 32)
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(lat + e * 128));
+                for (int e = lane; e < rows; e += 32)
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(rope + e * 128));
+            }
         }
     }
 }
@@ -580,45 +696,43 @@ __device__ __forceinline__ void value_output(const TreeArgs &a, TreeWalk walk, u
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int q4 = warp & 3, grp = (warp - 2) >> 2;
     const int row = 32 * q4 + lane;
-    const uint32_t oaddr = tbase + ((uint32_t)(32 * q4) << 16) + 128 * grp;
-    int g = 0, i = 0;
+    const uint32_t oaddr = tbase + ((uint32_t)(32 * q4) << 16) + TT_OW * grp;
+    const float *fac = reinterpret_cast<const float *>(sm + TT_OFF_F) + row;
+    int g = 0;
     TreeSeg sg, old;
     while (walk.next(sg)) {
         for (int t = sg.t0; t < sg.t1; t++, g++) {
             const int pb = g & 1, before = (g - 1) & 1, ph = ((g - 1) >> 1) & 1;
-            if (warp == 2 && lane == 0) mbar_expect_tx(&bars.p_in[pb], TT_P_BYTES);
+            if (warp == 2 && lane == 0) mbar_expect_tx(&bars.p_in[pb], TT_PBUF + TT_M * 4);
             if (t == sg.t0 && g > 0) {  // the last row tile's o, before it is written over
-                if (!lane_wait(&bars.pv_done[before], ph, a.err, 0x551)) return;
+                if (!warp_spin(&bars.pv_done[before], ph, a.err, 0x551)) return;
                 tc_fence_after();
-                write_o(a, old, cl, oaddr, row, 128 * grp, 128);
+                write_o(a, old, cl, oaddr, row, TT_OW * grp, TT_OW);
             }
-            if (!lane_wait<true>(&bars.p_in[pb], (g >> 1) & 1, a.err, 0x552)) return;
-            const float f = t == sg.t0 ? 1.f : bars.fac[pb][row];
+            if (!warp_spin<true>(&bars.p_in[pb], (g >> 1) & 1, a.err, 0x552)) return;
+            if (warp == 2 && lane == 0) mbar_arrive_cluster_relaxed(&bars.p_ack, 0);
+            const float f = t == sg.t0 ? 1.f : fac[pb * TT_M];
             if (__any_sync(0xffffffffu, f != 1.f)) {
-                if (!lane_wait(&bars.pv_done[before], ph, a.err, 0x553)) return;
+                if (!warp_spin(&bars.pv_done[before], ph, a.err, 0x553)) return;
                 tc_fence_after();
-                rescale_o(oaddr, 128, f);
+                rescale_o(oaddr, TT_OW, f);
             }
-            fence_async_shared();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.p_full[pb]);
-            if ((long long)(t + 1) * TT_TILE <= sg.s.len) {
-                i += TT_CHUNKS;
-                continue;
-            }
+            if ((long long)(t + 1) * TT_TILE <= sg.s.len) continue;
             // rows past the cached ones: zero where nothing is written, and where a draft's element
             // is not finite
-            for (int c = 0; c < TT_CHUNKS; c++, i++) {
-                const int st = i % TT_NST;
-                if (!lane_wait(&bars.full[st], (i / TT_NST) & 1, a.err, 0x554)) return;
+            for (int c = 0; c < TT_VCH; c++) {
+                if (!warp_spin(&bars.full[c], g & 1, a.err, 0x554)) return;
                 const long long d0 = sg.s.len - ((long long)t * TT_TILE + c * TT_VROWS);
                 const long long d1 = d0 + sg.s.n;
-                uint8_t *kv = sm + st * TT_VSTAGE;
+                uint8_t *kv = sm + c * TT_VSTAGE;
                 for (int e = threadIdx.x - 64; e < TT_VROWS * 64; e += TT_WORKERS * 32) {
                     const int r = e / 64, kb = (e / 8) % 8, ch = e % 8;
                     if (r < d0) continue;
-                    uint4 *p = reinterpret_cast<uint4 *>(kv + kb * TT_VBLK + r * 128 + ch * 16);
+                    uint4 *p = reinterpret_cast<uint4 *>(kv + (r / 8) * 8192 + kb * 1024 +
+                                                         (r % 8) * 128 + ch * 16);
                     uint4 w = make_uint4(0, 0, 0, 0);
                     if (r < d1) {
                         w = *p;
@@ -634,9 +748,9 @@ __device__ __forceinline__ void value_output(const TreeArgs &a, TreeWalk walk, u
         }
         old = sg;
     }
-    if (g > 0 && lane_wait(&bars.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, a.err, 0x555)) {
+    if (g > 0 && warp_spin(&bars.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, a.err, 0x555)) {
         tc_fence_after();
-        write_o(a, old, cl, oaddr, row, 128 * grp, 128);
+        write_o(a, old, cl, oaddr, row, TT_OW * grp, TT_OW);
     }
 }
 
@@ -655,21 +769,24 @@ mla_tree_attend_tc(const __grid_constant__ TreeMaps maps, const __grid_constant_
     if (cl >= G) return;  // both CTAs of the pair
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < TT_NST; s++) {
-            mbar_init(&bars.full[s], 1);
-            mbar_init(&bars.empty[s], 1);
+        for (int c = 0; c < TT_KCH; c++) {
+            mbar_init(&bars.full[c], 1);
+            mbar_init(&bars.empty[c], 1);
         }
+        for (int c = 0; c < TT_VCH; c++) mbar_init(&bars.clean[c], TT_WORKERS);
         mbar_init(&bars.q_full, TT_WORKERS);
         mbar_init(&bars.q_empty, 1);
-        mbar_init(&bars.s_full, 1);
-        mbar_init(&bars.s_empty, TT_WORKERS);
-        for (int q = 0; q < 4; q++) mbar_init(&bars.pair[q], 4);
+        for (int q = 0; q < 4; q++) mbar_init(&bars.pair[q], TT_GRP);
+        mbar_init(&bars.p_out, TT_WORKERS);
+        mbar_init(&bars.p_ack, 1);
         for (int b = 0; b < 2; b++) {
+            mbar_init(&bars.s_full[b], 1);
+            mbar_init(&bars.s_empty[b], TT_WORKERS);
             mbar_init(&bars.p_in[b], 1);
             mbar_init(&bars.p_full[b], TT_WORKERS);
             mbar_init(&bars.pv_done[b], 1);
         }
-        for (int c = 0; c < TT_CHUNKS; c++) mbar_init(&bars.clean[c], TT_WORKERS);
+        bars.tile = -1;
         fence_barrier_init();
     }
     if (warp == 1) tmem_alloc(&bars.tmem_base, TT_TM_COLS);
@@ -681,15 +798,15 @@ mla_tree_attend_tc(const __grid_constant__ TreeMaps maps, const __grid_constant_
     const TreeWalk walk(a, cl, total, G);
 
     if (warp == 0) {
-        if (lane == 0) prefetch_tmap(&maps.lat);
-        if (score) score_loads(maps, a, walk, sm, bars);
-        else value_loads(maps, a, walk, sm, bars);
+        if (lane == 0) prefetch_tmap(score ? &maps.lat_k : &maps.lat_v);
+        if (score) tree_loads<true>(maps, a, walk, sm, bars);
+        else tree_loads<false>(maps, a, walk, sm, bars);
     } else if (warp == 1) {
-        if (lane == 0) {
-            if (score) score_mma(a, walk, sm, bars, tbase);
-            else value_mma(a, walk, sm, bars, tbase);
-        }
-        __syncwarp();
+        if (score) score_mma(a, walk, sm, bars, tbase);
+        else value_mma(a, walk, sm, bars, tbase);
+    } else if (warp == 2 + TT_WORKERS) {
+        if (score) score_send(a, walk, sm, bars);
+        else value_prefetch(a, walk, bars);
     } else if (score) {
         score_softmax(a, walk, sm, bars, tbase, cl);
     } else {
@@ -701,64 +818,59 @@ mla_tree_attend_tc(const __grid_constant__ TreeMaps maps, const __grid_constant_
     if (warp == 1) tmem_dealloc(tbase, TT_TM_COLS);
 }
 
-// Join a row tile that several clusters took (the flash-decoding identity), for the cluster in
-// which it begins: one block per (cluster, row), thread t owns latent dims 4 t .. 4 t + 3.
+// Join the row tiles that several clusters took (the flash-decoding identity): block (c, y) takes
+// rows y, y + TT_JOIN, .. of the one that begins in cluster c; thread t owns latent dims 4 t .. 4 t + 3.
+constexpr int TT_JOIN = 32;
 __global__ void __launch_bounds__(128) mla_tree_join(const __grid_constant__ TreeArgs a) {
     pdl_trigger();
     pdl_wait();
-    const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, G = a.plan->G;
-    const long long total = a.plan->total;
-    if (c + 1 >= G) return;
-    // the row tile that holds the cluster's last place
-    const long long end = line_begin(total, G, c + 1);
-    const int b = last_at_most(a.cum, a.v.B, end - 1);
-    const PagedSeq s = paged_seq(a.v, b, K3CUDA_MAX_DRAFTS);
-    const long long cost = TT_FIXED + (s.len + s.n + TT_TILE - 1) / TT_TILE;
-    const int mt = (int)((end - 1 - a.cum[b]) / cost);
-    const long long first = a.cum[b] + mt * cost + TT_FIXED, last = first + cost - TT_FIXED - 1;
-    // cut here, with its first tile in this cluster
-    if (end <= first || last < end || first < line_begin(total, G, c)) return;
-    const int lr = mt * TT_M + row;
-    if (lr >= s.n * a.H) return;
-    const int cn = line_cluster(total, G, last);
-    const float *base = a.part + (size_t)row * TT_PART;
+    const int c = blockIdx.x, tid = threadIdx.x;
+    const TreeCut cut = a.plan->cut[c];
+    if (cut.last < 0) return;
     const size_t stride = (size_t)2 * TT_M * TT_PART;  // between clusters
-    auto part = [&](int k) { return base + k * stride + (k == c ? TT_M * TT_PART : 0); };
-    float M = -INFINITY;
-    for (int k = c; k <= cn; k++) M = fmaxf(M, part(k)[TT_DL]);
-    float L = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k0 = c; k0 <= cn; k0 += 4) {
-        float4 v[4];
-        float w[4], pl[4];
+    for (int row = blockIdx.y; row < cut.rows; row += TT_JOIN) {
+        const float *base = a.part + (size_t)row * TT_PART;
+        auto part = [&](int k) { return base + k * stride + (k == c ? TT_M * TT_PART : 0); };
+        float M = -INFINITY;
+        for (int k = c; k <= cut.last; k++) M = fmaxf(M, part(k)[TT_DL]);
+        float L = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k0 = c; k0 <= cut.last; k0 += 4) {
+            float4 v[4];
+            float w[4], pl[4];
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            w[u] = pl[u] = 0.f;
-            v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (k0 + u <= cn) {
-                const float *p = part(k0 + u);
-                const float m = p[TT_DL];
-                pl[u] = p[TT_DL + 1];
-                w[u] = m == -INFINITY && pl[u] == 0.f ? 0.f : exp2f(m - M);
-                v[u] = reinterpret_cast<const float4 *>(p)[tid];
+            for (int u = 0; u < 4; u++) {
+                w[u] = pl[u] = 0.f;
+                v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (k0 + u <= cut.last) {
+                    const float *p = part(k0 + u);
+                    const float m = p[TT_DL];
+                    pl[u] = p[TT_DL + 1];
+                    w[u] = m == -INFINITY && pl[u] == 0.f ? 0.f : exp2f(m - M);
+                    v[u] = reinterpret_cast<const float4 *>(p)[tid];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                L += w[u] * pl[u];
+                o.x += w[u] * v[u].x;
+                o.y += w[u] * v[u].y;
+                o.z += w[u] * v[u].z;
+                o.w += w[u] * v[u].w;
             }
         }
+        const float ov[4] = {o.x, o.y, o.z, o.w};
+        float lo[4];
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            L += w[u] * pl[u];
-            o.x += w[u] * v[u].x; o.y += w[u] * v[u].y; o.z += w[u] * v[u].z; o.w += w[u] * v[u].w;
-        }
+        for (int i = 0; i < 4; i++) lo[i] = ov[i] - __bfloat162float(__float2bfloat16_rn(ov[i]));
+        const size_t th = (size_t)cut.row0 + row;
+        __nv_bfloat16 *dst = a.olat2 + th * 2 * TT_DL;
+        reinterpret_cast<uint2 *>(dst)[tid] =
+            make_uint2(pack_bf2(ov[0], ov[1]), pack_bf2(ov[2], ov[3]));
+        reinterpret_cast<uint2 *>(dst + TT_DL)[tid] =
+            make_uint2(pack_bf2(lo[0], lo[1]), pack_bf2(lo[2], lo[3]));
+        if (tid == 0) a.rowsum[th] = L;
     }
-    const float ov[4] = {o.x, o.y, o.z, o.w};
-    float lo[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) lo[i] = ov[i] - __bfloat162float(__float2bfloat16_rn(ov[i]));
-    const size_t th = (size_t)s.first * a.H + lr;
-    __nv_bfloat16 *dst = a.olat2 + th * 2 * TT_DL;
-    reinterpret_cast<uint2 *>(dst)[tid] = make_uint2(pack_bf2(ov[0], ov[1]), pack_bf2(ov[2], ov[3]));
-    reinterpret_cast<uint2 *>(dst + TT_DL)[tid] =
-        make_uint2(pack_bf2(lo[0], lo[1]), pack_bf2(lo[2], lo[3]));
-    if (tid == 0) a.rowsum[th] = L;
 }
 
 static int tree_shape(int B, int T, int H, int dn, int dr, int dl, int dv) {
@@ -838,15 +950,19 @@ extern "C" int k3cuda_mla_tree_attend(k3cuda_ctx *ctx, void *out, int out_dtype,
     long long *cum = (long long *)(w + ws.cum);
     int *keep = (int *)(w + ws.keep);
     __nv_bfloat16 *qlat = (__nv_bfloat16 *)(w + ws.qlat);
-    const TreeArgs a{paged_view(cache, batch), plan, cum, tree_mask, qlat,
+    const TreeArgs a{paged_view(cache, batch), plan, cum, tree_mask,
+                     (const __nv_bfloat16 *)cache->latent, (const __nv_bfloat16 *)cache->rope, qlat,
                      (float *)(w + ws.part), (__nv_bfloat16 *)(w + ws.olat2),
                      (float *)(w + ws.rowsum), H, scale * 1.4426950408889634f, ctx->err_word};
     const uint64_t rows = (uint64_t)cache->n_pages * cache->page_size;
-    const uint32_t box = cache->page_size < TT_BOX ? cache->page_size : TT_BOX;
-    const CUtensorMapDataType BF = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const uint32_t kbox = cache->page_size < TT_TILE ? cache->page_size : TT_TILE;
+    const uint32_t vbox = cache->page_size < TT_VROWS ? cache->page_size : TT_VROWS;
     TreeMaps maps;
-    rc = make_tmap_2d(&maps.lat, cache->latent, BF, 2, TT_DL, rows, TT_DL * 2, 64, box);
-    if (!rc) rc = make_tmap_2d(&maps.rope, cache->rope, BF, 2, TT_DR, rows, TT_DR * 2, 64, box);
+    rc = make_tmap_rows8(&maps.lat_k, cache->latent, TT_DL, rows, TT_DL / 64 / TT_KCH, kbox);
+    if (!rc) rc = make_tmap_rows8(&maps.lat_v, cache->latent, TT_DL, rows, TT_DL / 64, vbox);
+    if (!rc)
+        rc = make_tmap_2d(&maps.rope, cache->rope, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, TT_DR, rows,
+                          TT_DR * 2, 64, kbox);
     if (rc || (rc = set_smem(mla_tree_attend_tc, TT_SMEM))) return rc;
 
     int clusters = ctx->sm_count / 2;
@@ -859,7 +975,7 @@ extern "C" int k3cuda_mla_tree_attend(k3cuda_ctx *ctx, void *out, int out_dtype,
         rc = launch_pdl(ctx, ctx->stream, "mla_tree_attend_tc", mla_tree_attend_tc,
                         dim3(2 * clusters), dim3(TT_THREADS), TT_SMEM, maps, a);
     if (!rc)
-        rc = launch_pdl(ctx, ctx->stream, "mla_tree_join", mla_tree_join, dim3(clusters, TT_M),
+        rc = launch_pdl(ctx, ctx->stream, "mla_tree_join", mla_tree_join, dim3(clusters, TT_JOIN),
                         dim3(128), 0, a);
     if (!rc)
         rc = mla_project(ctx, out, out_dtype, a.olat2, a.rowsum, keep, w_uv, TT_DV, T, H);

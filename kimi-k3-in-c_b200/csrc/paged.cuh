@@ -34,6 +34,7 @@ struct PagedView {
     const int *lens;    // [B]
     const int *cu;      // [B + 1]
     int B, T;
+    int shift;          // log2 of page_size
 };
 
 // Sequence b's new tokens: rows first .. first + n - 1 of the token arrays, behind `len` cached
@@ -60,10 +61,9 @@ K3_HD PagedSeq paged_seq(const PagedView &v, int b, int max_n) {
 // The cache row of sequence b's position pos (0 <= pos < max_pages * page_size, as paged_seq
 // has checked), or -1 where the table names a page that the cache does not have.
 K3_HD long long paged_row(const PagedView &v, int b, int pos) {
-    const int slot = pos / v.page_size;
-    const int page = v.table[(long long)b * v.max_pages + slot];
+    const int page = v.table[(long long)b * v.max_pages + (pos >> v.shift)];
     if (page < 0 || page >= v.n_pages) return -1;
-    return (long long)page * v.page_size + (pos - slot * v.page_size);
+    return ((long long)page << v.shift) + (pos & (v.page_size - 1));
 }
 
 // Work line of the tree attention. Every (sequence, row tile) is a unit that takes `fixed` +

@@ -103,6 +103,19 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t *bar, uint32_t pa
     return ok != 0;
 }
 
+// Whether the phase has completed, without waiting (try_wait sleeps for some microseconds first).
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 constexpr long long kWaitCycles = 1ll << 31;
 
 // The error block of a context (256 bytes of device memory): word 0 holds the code of the
@@ -143,6 +156,33 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, unsign
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity, unsigned *err,
                                                   unsigned code) {
     return mbar_wait_impl<true>(bar, parity, err, code);
+}
+
+// Bounded wait for short hand-offs: as mbar_wait, but nothing is read from global memory before 64
+// tries have failed. (mbar_wait reads the bound after the first try: a wait that just misses costs
+// an L2 round trip, 600 cycles, which a chain of hand-offs pays at every step.)
+template <bool kCluster = false>
+__device__ __forceinline__ bool mbar_spin(uint64_t *bar, uint32_t parity, unsigned *err,
+                                          unsigned code) {
+    if (kCluster ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    for (uint32_t i = 1;; i++) {
+        if (kCluster ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
+        if ((i & 63) == 0) {
+            if (*(volatile unsigned *)err) return false;
+            if (clock64() - t0 > wait_limit(err)) {
+                atomicCAS(err, 0u, code);
+                return false;
+            }
+        }
+    }
+}
+// The same by a whole warp; true only if every lane's wait completed.
+template <bool kCluster = false>
+__device__ __forceinline__ bool warp_spin(uint64_t *bar, uint32_t parity, unsigned *err,
+                                          unsigned code) {
+    const bool ok = mbar_spin<kCluster>(bar, parity, err, code);
+    return __all_sync(0xffffffffu, ok);
 }
 
 // Bounded wait by a whole warp; true only if every lane's wait completed.
@@ -201,6 +241,17 @@ __device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t b
         : "memory");
 }
 
+// Untiled bulk copy of `bytes` (a multiple of 16) from this CTA's shared memory into the shared
+// memory of another CTA of the cluster, completing on a barrier there (both from map_peer).
+__device__ __forceinline__ void bulk_send(uint32_t rdst, uint32_t src, uint32_t bytes,
+                                          uint32_t rbar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, "
+        "[%3];" ::"r"(rdst),
+        "r"(src), "r"(bytes), "r"(rbar)
+        : "memory");
+}
+
 // 2-D tiled load of box (c0 = inner, c1 = outer) into shared memory, completing on `bar`
 // (transaction bytes). The destination is this CTA's own shared memory.
 __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, uint64_t *bar,
@@ -218,6 +269,15 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, u
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
         "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
         "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, uint64_t *bar,
+                                            int c0, int c1, int c2, int c3) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+        "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
         : "memory");
 }
 
@@ -249,6 +309,13 @@ __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap *map, int c0, 
     asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(
                      (uint64_t)map),
                  "r"(c0), "r"(c1)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap *map, int c0, int c1, int c2,
+                                                int c3) {
+    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(
+                     (uint64_t)map),
+                 "r"(c0), "r"(c1), "r"(c2), "r"(c3)
                  : "memory");
 }
 __device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap *map, int c0, int c1, int c2) {
@@ -318,18 +385,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *v) {
     for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
 }
 
-// As tmem_ld16, 8 consecutive columns.
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float *v) {
-    uint32_t r[8];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7])
-        : "r"(taddr));
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = __uint_as_float(r[i]);
-}
-
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&v)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
@@ -351,7 +406,7 @@ __device__ __forceinline__ void tmem_wait_st() {
 }
 
 // ----------------------------------------------------------------------- descriptors
-constexpr uint32_t kSw128 = 2, kSw64 = 4;  // layout types: 128- and 64-byte swizzle
+constexpr uint32_t kSw128 = 2;  // layout type: 128-byte swizzle
 
 // Shared-memory matrix descriptor (start, leading and stride byte offsets, SW128).
 __device__ __forceinline__ uint64_t sdesc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
@@ -362,13 +417,6 @@ __device__ __forceinline__ uint64_t sdesc(uint32_t saddr, uint32_t lbo, uint32_t
 // K-major SW128 operand at `saddr` (1024-aligned region of rows x 128 B): the K step of
 // 16 bf16 (or 8 tf32) is +32 B on the start address.
 __device__ __forceinline__ uint64_t sdesc_kmajor(uint32_t saddr) { return sdesc(saddr, 16, 1024); }
-
-// K-major operand of 32 bf16 per row with the 64-byte swizzle (rows x 64 B, 512-aligned region:
-// eight rows form an atom, 16-byte chunk c of row r sits at c ^ ((r >> 1) & 3)).
-__device__ __forceinline__ uint64_t sdesc_kmajor64(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFF) | (1ull << 16) | ((uint64_t)(512 >> 4) << 32) |
-           (1ull << 46) | ((uint64_t)kSw64 << 61);
-}
 
 // MN-major SW128 operand: `mn_stride` bytes between consecutive 64-wide M/N blocks.
 __device__ __forceinline__ uint64_t sdesc_mnmajor(uint32_t saddr, uint32_t mn_stride) {
@@ -414,11 +462,45 @@ __device__ __forceinline__ void mma_commit(uint64_t *bar) {
                  : "memory");
 }
 
-// As mma_commit, arriving on the barrier at the same shared offset of every CTA in `mask`.
-__device__ __forceinline__ void mma_commit_cluster(uint64_t *bar, uint16_t mask) {
+// The same instructions taken by a whole converged warp: one elected lane issues them (always the
+// same one, so that a commit follows what it issued). Operands that are the same in every lane
+// stay in uniform registers; issued from a one-thread branch each MMA cost about 60 cycles
+// whatever its N (measured), in this form 23 at N = 32, 37 at N = 64, 74 at N = 128 (A in TMEM).
+__device__ __forceinline__ void warp_mma_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                            uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
-        "[%0], %1;" ::"r"(smem_u32(bar)),
+        "{\n\t.reg .pred p, e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void warp_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
+                                            uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void warp_commit(uint64_t *bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+            smem_u32(bar))
+        : "memory");
+}
+// Arrives on the barrier at the same shared offset of every CTA in `mask`.
+__device__ __forceinline__ void warp_commit_cluster(uint64_t *bar, uint16_t mask) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;\n\t}" ::"r"(smem_u32(bar)),
         "h"(mask)
         : "memory");
 }
@@ -455,14 +537,6 @@ __device__ __forceinline__ void st_async_v4(uint32_t raddr, float a, float b, fl
     asm volatile(
         "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::
             "r"(raddr), "f"(a), "f"(b), "f"(c), "f"(d), "r"(rbar)
-        : "memory");
-}
-
-// As st_async_v4, four bytes.
-__device__ __forceinline__ void st_async_f32(uint32_t raddr, float a, uint32_t rbar) {
-    asm volatile(
-        "st.async.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(raddr),
-        "f"(a), "r"(rbar)
         : "memory");
 }
 

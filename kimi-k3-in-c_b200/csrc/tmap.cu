@@ -14,8 +14,8 @@ namespace k3 {
 // time that a decode step repeats for the same tensors every call.
 struct TmapKey {
     const void *base;
-    uint64_t dims[3], strides[2];
-    uint32_t rank, dtype, elem, box[3];
+    uint64_t dims[4], strides[3];
+    uint32_t rank, dtype, elem, box[4];
 };
 struct TmapEntry {
     TmapKey key;
@@ -88,9 +88,8 @@ int make_tmap_2d(CUtensorMap *map, const void *base, CUtensorMapDataType dtype,
     cuuint64_t strides[1] = {row_bytes};
     cuuint32_t box[2] = {box_inner, box_outer};
     cuuint32_t estr[2] = {1, 1};
-    const CUtensorMapSwizzle sw = box_inner * elem_bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
-                                  : box_inner * elem_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                                                 : CU_TENSOR_MAP_SWIZZLE_NONE;
+    const CUtensorMapSwizzle sw = box_inner * elem_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                                                : CU_TENSOR_MAP_SWIZZLE_NONE;
     CUresult r = fn(map, dtype, 2, const_cast<void *>(base), dims, strides, box, estr,
                     CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -120,6 +119,28 @@ int make_tmap_3d(CUtensorMap *map, const void *base, CUtensorMapDataType dtype,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
         return set_error(K3CUDA_ERR_CUDA, "cuTensorMapEncodeTiled(3d) failed: %d", (int)r);
+    tmap_store(key, *map);
+    return K3CUDA_OK;
+}
+
+int make_tmap_rows8(CUtensorMap *map, const void *base, uint64_t inner, uint64_t rows,
+                    uint32_t box_blocks, uint32_t box_rows) {
+    const uint64_t kd[4] = {64, 8, inner / 64, rows / 8}, ks[3] = {inner * 2, 128, inner * 16};
+    const uint32_t kb[4] = {64, 8, box_blocks, box_rows / 8};
+    const CUtensorMapDataType BF = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const TmapKey key = tmap_key(4, base, BF, 2, kd, ks, kb);
+    if (tmap_lookup(key, map)) return K3CUDA_OK;
+    auto fn = encode_fn();
+    if (!fn) return set_error(K3CUDA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+    cuuint64_t dims[4] = {kd[0], kd[1], kd[2], kd[3]};
+    cuuint64_t strides[3] = {ks[0], ks[1], ks[2]};
+    cuuint32_t box[4] = {kb[0], kb[1], kb[2], kb[3]};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = fn(map, BF, 4, const_cast<void *>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return set_error(K3CUDA_ERR_CUDA, "cuTensorMapEncodeTiled(4d) failed: %d", (int)r);
     tmap_store(key, *map);
     return K3CUDA_OK;
 }

@@ -179,13 +179,13 @@ int main() {
     auto rnd = [&](int lo, int hi) { return (int)(lo + (long long)(g() % (unsigned)((long long)hi - lo + 1))); };
     // tables that hold anything: no index ever leaves the arrays
     for (int it = 0; it < 20000; it++) {
-        const int B = rnd(1, 6), mp = rnd(1, 5), ps = 8 << rnd(0, 4), np = rnd(1, 9), T = rnd(0, 40);
+        const int B = rnd(1, 6), mp = rnd(1, 5), sh = rnd(3, 7), ps = 1 << sh, np = rnd(1, 9), T = rnd(0, 40);
         const bool wild = it & 1;
         std::vector<int> table(B * mp), lens(B), cu(B + 1);
         for (int &x : table) x = wild && rnd(0, 3) == 0 ? (int)g() : rnd(0, np - 1);
         for (int &x : lens) x = wild && rnd(0, 3) == 0 ? (int)g() : rnd(0, mp * ps);
         for (int i = 0; i <= B; i++) cu[i] = wild && rnd(0, 3) == 0 ? (int)g() : (i ? cu[i - 1] : 0) + rnd(0, 9);
-        const PagedView v{table.data(), np, ps, mp, lens.data(), cu.data(), B, T};
+        const PagedView v{table.data(), np, ps, mp, lens.data(), cu.data(), B, T, sh};
         for (int b = 0; b < B; b++) {
             const PagedSeq s = paged_seq(v, b, 64);
             assert(s.n >= 0 && (s.n == 0 || (s.first >= 0 && s.first + s.n <= T && s.len >= 0)));
@@ -205,7 +205,7 @@ int main() {
     }
     // offsets past 32 bits of elements
     { int table[1] = {(1 << 27) - 1}, len[1] = {5}, cu[2] = {0, 1};
-      const PagedView v{table, 1 << 27, 8, 1, len, cu, 1, 1};
+      const PagedView v{table, 1 << 27, 8, 1, len, cu, 1, 1, 3};
       assert(paged_row(v, 0, 7) == (1ll << 30) - 1); }
     // the work line: every place lies in the cluster that line_cluster names
     for (int it = 0; it < 3000; it++) {

@@ -332,8 +332,9 @@ def test_tree_split_contexts(ctx, B, n, H, ctx_len):
 
 def test_tree_scores_far_apart(ctx):
     """Scores that grow by thousands along the context (the running maximum moves late), and a
-    scale of either sign."""
+    scale of zero and of either sign."""
     rng = np.random.default_rng(9)
+    check_tree(ctx, rng, [300, 0], [3, 2], 16, 5, "tree", scale=0.0)
     for scale in (0.0722, -0.0722):
         p = Paged(ctx, rng, [500, 70], [4, 2], 16)
         p.fill_drafts(rng)
