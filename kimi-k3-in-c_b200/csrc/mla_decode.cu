@@ -194,6 +194,21 @@ __device__ __forceinline__ float row_factor(const float *rowsum, size_t row) {
     return l == 0.f ? 0.f : 1.f / l;
 }
 
+// 16 values times f, 16 bytes a store
+__device__ __forceinline__ void store16(float *p, const float *v, float f) {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        reinterpret_cast<float4 *>(p)[i] =
+            make_float4(v[4 * i] * f, v[4 * i + 1] * f, v[4 * i + 2] * f, v[4 * i + 3] * f);
+}
+__device__ __forceinline__ void store16(__nv_bfloat16 *p, const float *v, float f) {
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) x[i] = v[i] * f;
+    reinterpret_cast<uint4 *>(p)[0] = pack_bf8(x);
+    reinterpret_cast<uint4 *>(p)[1] = pack_bf8(x + 8);
+}
+
 // rowsum: see row_factor; keep [B]: rows of 0 are not stored (NULL: every row is)
 template <typename OUT>
 __global__ void __launch_bounds__(128, 2)
@@ -262,14 +277,19 @@ mla_project_tc(const __grid_constant__ HeadGemmMaps maps, OUT *__restrict__ out,
     if (ok) {
         const bool st = b < B && (!keep || keep[b]);
         const float f = st ? row_factor(rowsum, (size_t)b * H + h) : 0.f;
+        const bool wide = ((uintptr_t)out & 15) == 0;  // rows are multiples of 16 bytes
         for (int c = 0; c < 128; c += 16) {
             float v[16];
             tmem_ld16(tb + ((uint32_t)(32 * warp) << 16) + c, v);
             tmem_wait_ld();
-            if (st)
+            if (!st) continue;
+            OUT *dst = out + ((size_t)b * H + h) * MLA_DV + c;
+            if (wide) {
+                store16(dst, v, f);
+            } else {
 #pragma unroll
-                for (int i = 0; i < 16; i++)
-                    io<OUT>::st(out + ((size_t)b * H + h) * MLA_DV + c + i, v[i] * f);
+                for (int i = 0; i < 16; i++) io<OUT>::st(dst + i, v[i] * f);
+            }
         }
     }
     tc_fence_before();

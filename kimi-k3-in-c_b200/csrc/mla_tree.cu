@@ -79,8 +79,13 @@ constexpr int TT_GRP = 2;                  // groups of worker warps, one warp p
 constexpr int TT_OFF_VAL = TT_OFF_FS + TT_M * 4;      // values shared by a row's warps
 constexpr int TT_OFF_P = TT_VCH * TT_VSTAGE;      // value: P, two buffers
 constexpr int TT_OFF_F = TT_OFF_P + 2 * TT_PBUF;  // and their factors
-constexpr int TT_SMEM = TT_OFF_VAL + 2 * TT_GRP * TT_M * 4 + 1024;
-static_assert(TT_OFF_F + 2 * TT_M * 4 <= TT_SMEM - 1024, "both CTAs' layouts fit");
+constexpr int TT_OFF_W = TT_OFF_F + 1024;         // o on its way out, 4 KB a warp
+constexpr int TT_OFF_QS = TT_OFF_VAL + 2 * TT_GRP * TT_M * 4;  // queries on their way in, 2 KB a warp
+constexpr int TT_SMEM_SCORE = TT_OFF_QS + 4 * TT_GRP * 2048;
+constexpr int TT_SMEM_VALUE = TT_OFF_W + 4 * TT_GRP * 4096;
+constexpr int TT_SMEM = (TT_SMEM_SCORE > TT_SMEM_VALUE ? TT_SMEM_SCORE : TT_SMEM_VALUE) + 1024;
+static_assert(TT_OFF_W % 1024 == 0 && 2 * TT_M * 4 <= 1024, "the stages are swizzled");
+
 constexpr int TT_TM_Q = 0, TT_TM_S = 256, TT_TM_COLS = 512;
 constexpr int TT_CW = TT_TILE / TT_GRP;    // score columns of a softmax warp
 constexpr int TT_OW = TT_DL / TT_GRP;      // dims of o of a warp in the value CTA
@@ -90,24 +95,31 @@ constexpr int TT_CLUSTERS = 74;            // 148 SMs of a B200
 constexpr int TT_FIXED = 4;                // a row tile's fixed work, in tiles
 constexpr int TT_MIN_TILES = 2;            // fewest tiles per cluster
 constexpr int TT_PART = TT_DL + 4;         // floats of a partial row: o, m, l, pad
-// A row tile that is cut and begins in some cluster: the last cluster with a part of it (-1: the
-// cluster begins none), its rows, and its first row among all (token, head) rows.
+// A row tile that is cut: the clusters with the first and the last part of it, its rows, and its first
+// row among all (token, head) rows.
 struct TreeCut {
-    int last, rows;
+    int first, last, rows;
     long long row0;
+};
+
+// Where a cluster's piece of the line begins: a row tile and its first place.
+struct TreeStart {
+    int b, mt;
+    long long at;
 };
 
 // the device-side plan, at the start of the workspace
 struct TreePlan {
     long long total;   // places on the line
     int G;             // clusters that take part
+    int cuts;
     TreeCut cut[TT_CLUSTERS];
+    TreeStart start[TT_CLUSTERS];
 };
 
 struct TreeArgs {
     PagedView v;
     const TreePlan *plan;
-    const long long *cum;      // [B + 1] first place of each sequence
     const unsigned long long *mask;
     const __nv_bfloat16 *latent, *rope;  // the cache's rows
     const __nv_bfloat16 *qlat; // [T][H][576]
@@ -146,10 +158,11 @@ struct TreeWalk {
     }
     __device__ __forceinline__ TreeWalk(const TreeArgs &args, int c, long long total, int G)
         : a(args), c0(line_begin(total, G, c)), c1(line_begin(total, G, c + 1)) {
-        b = last_at_most(a.cum, a.v.B, c0);
+        const TreeStart first = a.plan->start[c];
+        b = first.b;
+        mt = first.mt;
+        at = first.at;
         seq();
-        mt = (int)((c0 - a.cum[b]) / cost);
-        at = a.cum[b] + mt * cost;
     }
     __device__ __forceinline__ bool next(TreeSeg &g) {
         while (at < c1) {
@@ -230,8 +243,19 @@ __global__ void __launch_bounds__(1024) mla_tree_plan(PagedView v, int H, TreePl
     // the row tile that holds each cluster's last place
     const int G = plan->G;
     const long long total = carry;
+    if (tid < G) {
+        TreeStart start;
+        const long long c0 = line_begin(total, G, tid);
+        start.b = last_at_most(cum, v.B, c0);
+        const PagedSeq s = paged_seq(v, start.b, K3CUDA_MAX_DRAFTS);
+        const long long cost = TT_FIXED + (s.len + s.n + TT_TILE - 1) / TT_TILE;
+        start.mt = (int)((c0 - cum[start.b]) / cost);
+        start.at = cum[start.b] + start.mt * cost;
+        plan->start[tid] = start;
+    }
+    __shared__ TreeCut cut[TT_CLUSTERS];
     if (tid < TT_CLUSTERS) {
-        TreeCut cut{-1, 0, 0};
+        cut[tid].last = -1;
         if (tid + 1 < G) {
             const long long end = line_begin(total, G, tid + 1);
             const int b = last_at_most(cum, v.B, end - 1);
@@ -241,12 +265,19 @@ __global__ void __launch_bounds__(1024) mla_tree_plan(PagedView v, int H, TreePl
             const long long first = cum[b] + mt * cost + TT_FIXED, last = first + cost - TT_FIXED - 1;
             // some of its tiles are in this cluster, the first among them, and some are not
             if (first < end && end <= last && first >= line_begin(total, G, tid)) {
-                cut.last = line_cluster(total, G, last);
-                cut.rows = min(TT_M, s.n * H - mt * TT_M);
-                cut.row0 = (long long)s.first * H + mt * TT_M;
+                cut[tid].first = tid;
+                cut[tid].last = line_cluster(total, G, last);
+                cut[tid].rows = min(TT_M, s.n * H - mt * TT_M);
+                cut[tid].row0 = (long long)s.first * H + mt * TT_M;
             }
         }
-        plan->cut[tid] = cut;
+    }
+    __syncthreads();
+    if (tid < TT_CLUSTERS) {
+        int at = 0;
+        for (int c = 0; c < tid; c++) at += cut[c].last >= 0;
+        if (cut[tid].last >= 0) plan->cut[at++] = cut[tid];
+        if (tid + 1 == TT_CLUSTERS) plan->cuts = at;
     }
 }
 
@@ -265,6 +296,7 @@ struct TreeBars {
 
 // n columns of o from addr: multiply by f
 __device__ __forceinline__ void rescale_o(uint32_t addr, int n, float f) {
+#pragma unroll 1
     for (int c = 0; c < n; c += 16) {
         float v[16];
         tmem_ld16(addr + c, v);
@@ -276,63 +308,120 @@ __device__ __forceinline__ void rescale_o(uint32_t addr, int n, float f) {
     tmem_wait_st();
 }
 
-// A segment's o, latent dims dim .. dim + n - 1 (TMEM columns from addr) of row `row`: to the
-// partial, or (a whole row tile) as the projection's bf16 hi/lo pair.
+// A segment's o, latent dims dim .. dim + n - 1 (TMEM columns from addr) of the warp's 32 rows from
+// row0: to the partial, or (a whole row tile) as the projection's bf16 hi/lo pair. A lane reads its
+// row from TMEM; the rows go through 4 KB of shared memory so that they are stored 64 or 128 bytes of
+// a row at a time (stored straight from the lanes, 16 bytes of 32 rows each, this took 20000 cycles).
+// Here and in load_q the loops stay rolled: what runs once per row tile is not in the instruction
+// cache, and every 128 bytes of it cost some 250 cycles.
 __device__ __forceinline__ void write_o(const TreeArgs &a, const TreeSeg &g, int cl, uint32_t addr,
-                                        int row, int dim, int n) {
-    const int lr = g.mt * TT_M + row;
-    const bool ok = lr < g.s.n * a.H, whole = g.whole();
-    const size_t th = (size_t)g.s.first * a.H + lr;
-    float *dst = a.part + ((size_t)g.slot(cl) * TT_M + row) * TT_PART + dim;
-    __nv_bfloat16 *hi = a.olat2 + th * 2 * TT_DL + dim;
-    for (int c = 0; c < n; c += 16) {
-        float v[16];
-        tmem_ld16(addr + c, v);
+                                        uint8_t *stage, int row0, int dim, int n) {
+    const int lane = threadIdx.x & 31, j = lane & 7;
+    const bool whole = g.whole();
+    const int rows = min(32, g.s.n * a.H - (g.mt * TT_M + row0));  // that exist
+    // this lane's 16-byte chunk of rows lane / 8, + 4, ..: of 32 fp32, or of 32 hi and 32 lo halves
+    char *dst;
+    size_t pitch, step;
+    if (whole) {
+        dst = reinterpret_cast<char *>(
+            a.olat2 + ((size_t)g.s.first * a.H + g.mt * TT_M + row0) * 2 * TT_DL + dim);
+        dst += (j & 3) * 16 + (j >> 2) * TT_DL * 2;
+        pitch = TT_DL * 4;
+        step = 64;
+    } else {
+        dst = reinterpret_cast<char *>(a.part + ((size_t)g.slot(cl) * TT_M + row0) * TT_PART + dim);
+        dst += j * 16;
+        pitch = TT_PART * 4;
+        step = 128;
+    }
+    dst += (lane >> 3) * pitch;
+#pragma unroll 1
+    for (int c = 0; c < n; c += 32, dst += step) {
+        float v[32];
+        tmem_ld32(addr + c, v);
         tmem_wait_ld();
-        if (!ok) continue;
-        if (!whole) {
-            float4 *d4 = reinterpret_cast<float4 *>(dst + c);
+        if (whole) {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                d4[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            for (int i = 0; i < 4; i++) {
+                const uint4 hi = pack_bf8(v + 8 * i);
+                float h[8], lo[8];
+                unpack_bf8(hi, h);
+#pragma unroll
+                for (int k = 0; k < 8; k++) lo[k] = v[8 * i + k] - h[k];
+                st16s(stage + swz(lane, i), hi);
+                st16s(stage + swz(lane, 4 + i), pack_bf8(lo));
+            }
         } else {
-            float lo[16];
 #pragma unroll
-            for (int i = 0; i < 16; i++)
-                lo[i] = v[i] - __bfloat162float(__float2bfloat16_rn(v[i]));
-            uint4 *h4 = reinterpret_cast<uint4 *>(hi + c), *l4 = h4 + TT_DL / 8;
-            h4[0] = pack_bf8(v);
-            h4[1] = pack_bf8(v + 8);
-            l4[0] = pack_bf8(lo);
-            l4[1] = pack_bf8(lo + 8);
+            for (int i = 0; i < 8; i++)
+                st16s(stage + swz(lane, i),
+                      make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]),
+                                 __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3])));
         }
+        __syncwarp();
+        char *d = dst;
+#pragma unroll
+        for (int i = 0; i < 8; i++, d += 4 * pitch) {
+            const int r = 4 * i + (lane >> 3);
+            if (r < rows)
+                *reinterpret_cast<uint4 *>(d) = *reinterpret_cast<const uint4 *>(stage + swz(r, j));
+        }
+        __syncwarp();
     }
 }
 
 // A row tile's queries: the latent dims into TMEM (lane = row, two bf16 per column), group grp of a
 // quarter one half of them; the rope dims into shared memory, 32 dims a group. Rows past the last
-// token's are zero.
+// token's are zero. A negative scale is taken by the queries' sign, and a scale of zero makes them
+// zero. A warp reads 64 bytes of 8 rows at a time and turns them round in 2 KB of shared memory.
 __device__ __forceinline__ void load_q(const TreeArgs &a, const TreeSeg &g, uint32_t lane_addr,
-                                       uint8_t *rope, int row, int grp) {
-    const int lr = g.mt * TT_M + row;
-    const bool ok = lr < g.s.n * a.H;
-    const uint4 *q = reinterpret_cast<const uint4 *>(a.qlat + ((size_t)g.s.first * a.H + lr) * TT_QW);
-    const uint4 none = make_uint4(0, 0, 0, 0);
+                                       uint8_t *stage, uint8_t *rope, int q4, int grp) {
+    const int lane = threadIdx.x & 31, r0 = 32 * q4, c = lane & 3;
+    const int rows = a.scale_log2e == 0.f ? 0 : min(32, g.s.n * a.H - (g.mt * TT_M + r0));
+    const uint32_t flip = a.scale_log2e < 0.f ? 0x80008000u : 0u;
+    const uint4 *q = reinterpret_cast<const uint4 *>(
+        a.qlat + ((size_t)g.s.first * a.H + g.mt * TT_M + r0 + (lane >> 2)) * TT_QW) + c;
+    // step k: 32 dims, the last the rope dims; rows 8 i + lane / 4, 16-byte chunk lane % 4
+    auto fetch = [&](uint4 (&w)[4], int k) {
+        const int dim = k < 8 ? 256 * grp + 32 * k : TT_DL + 32 * grp;
 #pragma unroll
-    for (int i = 4 * grp; i < 4 * grp + 4; i++)
-        st16s(rope + swz(row, i), ok ? q[TT_DL / 8 + i] : none);
-    for (int h = 8 * grp; h < 8 * grp + 8; h++) {  // half blocks: 32 dims, 16 columns
+        for (int i = 0; i < 4; i++) {
+            w[i] = make_uint4(0, 0, 0, 0);
+            if (8 * i + (lane >> 2) < rows) {
+                const uint4 x = q[i * TT_QW + dim / 8];  // 8 rows of TT_QW / 8
+                w[i] = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
+            }
+        }
+    };
+    auto at = [&](int r, int ch) { return stage + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4); };
+    uint4 w[4], next[4], after[4];
+    fetch(w, 0);
+    fetch(next, 1);
+#pragma unroll 1
+    for (int k = 0; k < 8; k++) {
+        fetch(after, k + 2 < 9 ? k + 2 : 8);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; i++) st16s(at(8 * i + (lane >> 2), c), w[i]);
+        __syncwarp();
         float v[16];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const uint4 w = ok ? q[4 * h + i] : none;
-            v[4 * i] = __uint_as_float(w.x);
-            v[4 * i + 1] = __uint_as_float(w.y);
-            v[4 * i + 2] = __uint_as_float(w.z);
-            v[4 * i + 3] = __uint_as_float(w.w);
+            const uint4 x = *reinterpret_cast<const uint4 *>(at(lane, i));
+            v[4 * i] = __uint_as_float(x.x);
+            v[4 * i + 1] = __uint_as_float(x.y);
+            v[4 * i + 2] = __uint_as_float(x.z);
+            v[4 * i + 3] = __uint_as_float(x.w);
         }
-        tmem_st16(lane_addr + TT_TM_Q + 16 * h, v);
+        tmem_st16(lane_addr + TT_TM_Q + 128 * grp + 16 * k, v);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            w[i] = next[i];
+            next[i] = after[i];
+        }
     }
+#pragma unroll
+    for (int i = 0; i < 4; i++) st16s(rope + swz(r0 + 8 * i + (lane >> 2), 4 * grp + c), w[i]);
     tmem_wait_st();
 }
 
@@ -480,9 +569,8 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
     uint8_t *P = sm + TT_OFF_PS + grp * (TT_M * 128);  // this warp's 64-column block
     float *val = reinterpret_cast<float *>(sm + TT_OFF_VAL) + row;  // [2][TT_GRP][TT_M]
     // Scores are scaled to log2 units with the maximum's subtraction, by a positive factor (a masked
-    // -inf stays one): a negative scale changes their sign first, a scale of zero makes them zero.
+    // -inf stays one): see load_q.
     const float scale = a.scale_log2e == 0.f ? 1.f : fabsf(a.scale_log2e);
-    const float sign = a.scale_log2e > 0.f ? 1.f : a.scale_log2e < 0.f ? -1.f : 0.f;
     float m_ref = -INFINITY, l = 0.f;  // l: this warp's columns
     int g = 0, nq = 0, np = 0;
     // the other warp's value of the row
@@ -501,7 +589,7 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
         // this warp's part of the queries (the last row tile's S must be done)
         if (nq > 0 && !warp_spin(&bars.q_empty, (nq - 1) & 1, a.err, 0x522)) return;
         tc_fence_after();
-        load_q(a, sg, laddr, sm + TT_OFF_QR, row, grp);
+        load_q(a, sg, laddr, sm + TT_OFF_QS + (warp - 2) * 2048, sm + TT_OFF_QR, q4, grp);
         fence_async_shared();
         tc_fence_before();
         __syncwarp();
@@ -515,26 +603,30 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
             float s[TT_CW];
             if (!warp_spin(&bars.s_full[sb], (g >> 1) & 1, a.err, 0x523)) return;
             tc_fence_after();
+            const int p0 = t * TT_TILE + c0;
+            if (p0 + TT_CW > sg.s.len) {  // reaches past the cached rows: masked in TMEM
+                const uint64_t see = tree_bits(word, sg.s.len, sg.s.n, p0);
+                const int d0 = sg.s.len - p0;
+#pragma unroll 1
+                for (int c = 0; c < TT_CW; c += 16) {
+                    float x[16];
+                    tmem_ld16(laddr + TT_TM_S + sb * TT_TILE + c0 + c, x);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        if (c + i >= d0 && !(fabsf(x[i]) < INFINITY)) x[i] = NAN;
+                        if (!((see >> (c + i)) & 1)) x[i] = -INFINITY;
+                    }
+                    tmem_st16(laddr + TT_TM_S + sb * TT_TILE + c0 + c, x);
+                }
+                tmem_wait_st();
+            }
             tmem_ld32(laddr + TT_TM_S + sb * TT_TILE + c0, s);
             tmem_ld32(laddr + TT_TM_S + sb * TT_TILE + c0 + 32, s + 32);
             tmem_wait_ld();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.s_empty[sb]);
-            if (sign != 1.f) {
-#pragma unroll
-                for (int i = 0; i < TT_CW; i++) s[i] *= sign;
-            }
-            const int p0 = t * TT_TILE + c0;
-            if (p0 + TT_CW > sg.s.len) {  // reaches past the cached rows
-                const uint64_t see = tree_bits(word, sg.s.len, sg.s.n, p0);
-                const int d0 = sg.s.len - p0;
-#pragma unroll
-                for (int i = 0; i < TT_CW; i++) {
-                    if (i >= d0 && !(fabsf(s[i]) < INFINITY)) s[i] = NAN;
-                    if (!((see >> i) & 1)) s[i] = -INFINITY;
-                }
-            }
             float m4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
             for (int i = 4; i < TT_CW; i += 8)
@@ -698,6 +790,7 @@ __device__ __forceinline__ void value_output(const TreeArgs &a, TreeWalk walk, u
     const int row = 32 * q4 + lane;
     const uint32_t oaddr = tbase + ((uint32_t)(32 * q4) << 16) + TT_OW * grp;
     const float *fac = reinterpret_cast<const float *>(sm + TT_OFF_F) + row;
+    uint8_t *stage = sm + TT_OFF_W + (warp - 2) * 4096;
     int g = 0;
     TreeSeg sg, old;
     while (walk.next(sg)) {
@@ -707,7 +800,7 @@ __device__ __forceinline__ void value_output(const TreeArgs &a, TreeWalk walk, u
             if (t == sg.t0 && g > 0) {  // the last row tile's o, before it is written over
                 if (!warp_spin(&bars.pv_done[before], ph, a.err, 0x551)) return;
                 tc_fence_after();
-                write_o(a, old, cl, oaddr, row, TT_OW * grp, TT_OW);
+                write_o(a, old, cl, oaddr, stage, 32 * q4, TT_OW * grp, TT_OW);
             }
             if (!warp_spin<true>(&bars.p_in[pb], (g >> 1) & 1, a.err, 0x552)) return;
             if (warp == 2 && lane == 0) mbar_arrive_cluster_relaxed(&bars.p_ack, 0);
@@ -750,7 +843,27 @@ __device__ __forceinline__ void value_output(const TreeArgs &a, TreeWalk walk, u
     }
     if (g > 0 && warp_spin(&bars.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, a.err, 0x555)) {
         tc_fence_after();
-        write_o(a, old, cl, oaddr, row, TT_OW * grp, TT_OW);
+        write_o(a, old, cl, oaddr, stage, 32 * q4, TT_OW * grp, TT_OW);
+    }
+}
+
+__device__ __forceinline__ void tree_roles(const TreeMaps &maps, const TreeArgs &a,
+                                           const TreeWalk &walk, uint8_t *sm, TreeBars &bars,
+                                           uint32_t tbase, int cl, bool score) {
+    const int warp = threadIdx.x >> 5;
+    if (warp == 0) {
+        if (score) tree_loads<true>(maps, a, walk, sm, bars);
+        else tree_loads<false>(maps, a, walk, sm, bars);
+    } else if (warp == 1) {
+        if (score) score_mma(a, walk, sm, bars, tbase);
+        else value_mma(a, walk, sm, bars, tbase);
+    } else if (warp == 2 + TT_WORKERS) {
+        if (score) score_send(a, walk, sm, bars);
+        else value_prefetch(a, walk, bars);
+    } else if (score) {
+        score_softmax(a, walk, sm, bars, tbase, cl);
+    } else {
+        value_output(a, walk, sm, bars, tbase, cl);
     }
 }
 
@@ -759,15 +872,10 @@ mla_tree_attend_tc(const __grid_constant__ TreeMaps maps, const __grid_constant_
     extern __shared__ uint8_t smraw[];
     uint8_t *sm = (uint8_t *)(((uintptr_t)smraw + 1023) & ~(uintptr_t)1023);
     __shared__ TreeBars bars;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5;
     const bool score = cluster_rank() == 0;
     const int cl = blockIdx.x >> 1;
     pdl_trigger();
-    pdl_wait();  // the plan, the queries and the cache come from earlier work
-    const long long total = a.plan->total;
-    const int G = a.plan->G;
-    if (cl >= G) return;  // both CTAs of the pair
-
     if (threadIdx.x == 0) {
         for (int c = 0; c < TT_KCH; c++) {
             mbar_init(&bars.full[c], 1);
@@ -788,6 +896,7 @@ mla_tree_attend_tc(const __grid_constant__ TreeMaps maps, const __grid_constant_
         }
         bars.tile = -1;
         fence_barrier_init();
+        prefetch_tmap(score ? &maps.lat_k : &maps.lat_v);
     }
     if (warp == 1) tmem_alloc(&bars.tmem_base, TT_TM_COLS);
     tc_fence_before();
@@ -795,40 +904,26 @@ mla_tree_attend_tc(const __grid_constant__ TreeMaps maps, const __grid_constant_
     cluster_sync();  // the peer's barriers are ready before anything arrives on them
     tc_fence_after();
     const uint32_t tbase = bars.tmem_base;
-    const TreeWalk walk(a, cl, total, G);
-
-    if (warp == 0) {
-        if (lane == 0) prefetch_tmap(score ? &maps.lat_k : &maps.lat_v);
-        if (score) tree_loads<true>(maps, a, walk, sm, bars);
-        else tree_loads<false>(maps, a, walk, sm, bars);
-    } else if (warp == 1) {
-        if (score) score_mma(a, walk, sm, bars, tbase);
-        else value_mma(a, walk, sm, bars, tbase);
-    } else if (warp == 2 + TT_WORKERS) {
-        if (score) score_send(a, walk, sm, bars);
-        else value_prefetch(a, walk, bars);
-    } else if (score) {
-        score_softmax(a, walk, sm, bars, tbase, cl);
-    } else {
-        value_output(a, walk, sm, bars, tbase, cl);
-    }
+    pdl_wait();  // the plan, the queries and the cache come from earlier work
+    const int G = a.plan->G;
+    if (cl < G) tree_roles(maps, a, TreeWalk(a, cl, a.plan->total, G), sm, bars, tbase, cl, score);
     tc_fence_before();
     __syncthreads();
     cluster_sync();  // nothing of the peer's is on its way into this CTA's shared memory
     if (warp == 1) tmem_dealloc(tbase, TT_TM_COLS);
 }
 
-// Join the row tiles that several clusters took (the flash-decoding identity): block (c, y) takes
-// rows y, y + TT_JOIN, .. of the one that begins in cluster c; thread t owns latent dims 4 t .. 4 t + 3.
-constexpr int TT_JOIN = 32;
+// Join the row tiles that several clusters took (the flash-decoding identity), a row per block and
+// round; thread t owns latent dims 4 t .. 4 t + 3.
 __global__ void __launch_bounds__(128) mla_tree_join(const __grid_constant__ TreeArgs a) {
     pdl_trigger();
     pdl_wait();
-    const int c = blockIdx.x, tid = threadIdx.x;
-    const TreeCut cut = a.plan->cut[c];
-    if (cut.last < 0) return;
+    const int tid = threadIdx.x, items = a.plan->cuts * TT_M;
     const size_t stride = (size_t)2 * TT_M * TT_PART;  // between clusters
-    for (int row = blockIdx.y; row < cut.rows; row += TT_JOIN) {
+    for (int i = blockIdx.x; i < items; i += gridDim.x) {
+        const TreeCut cut = a.plan->cut[i / TT_M];
+        const int row = i % TT_M, c = cut.first;
+        if (row >= cut.rows) continue;
         const float *base = a.part + (size_t)row * TT_PART;
         auto part = [&](int k) { return base + k * stride + (k == c ? TT_M * TT_PART : 0); };
         float M = -INFINITY;
@@ -950,7 +1045,7 @@ extern "C" int k3cuda_mla_tree_attend(k3cuda_ctx *ctx, void *out, int out_dtype,
     long long *cum = (long long *)(w + ws.cum);
     int *keep = (int *)(w + ws.keep);
     __nv_bfloat16 *qlat = (__nv_bfloat16 *)(w + ws.qlat);
-    const TreeArgs a{paged_view(cache, batch), plan, cum, tree_mask,
+    const TreeArgs a{paged_view(cache, batch), plan, tree_mask,
                      (const __nv_bfloat16 *)cache->latent, (const __nv_bfloat16 *)cache->rope, qlat,
                      (float *)(w + ws.part), (__nv_bfloat16 *)(w + ws.olat2),
                      (float *)(w + ws.rowsum), H, scale * 1.4426950408889634f, ctx->err_word};
@@ -975,7 +1070,7 @@ extern "C" int k3cuda_mla_tree_attend(k3cuda_ctx *ctx, void *out, int out_dtype,
         rc = launch_pdl(ctx, ctx->stream, "mla_tree_attend_tc", mla_tree_attend_tc,
                         dim3(2 * clusters), dim3(TT_THREADS), TT_SMEM, maps, a);
     if (!rc)
-        rc = launch_pdl(ctx, ctx->stream, "mla_tree_join", mla_tree_join, dim3(clusters, TT_JOIN),
+        rc = launch_pdl(ctx, ctx->stream, "mla_tree_join", mla_tree_join, dim3(8 * ctx->sm_count),
                         dim3(128), 0, a);
     if (!rc)
         rc = mla_project(ctx, out, out_dtype, a.olat2, a.rowsum, keep, w_uv, TT_DV, T, H);
