@@ -80,8 +80,7 @@ constexpr int TT_OFF_VAL = TT_OFF_FS + TT_M * 4;      // values shared by a row'
 constexpr int TT_OFF_P = TT_VCH * TT_VSTAGE;      // value: P, two buffers
 constexpr int TT_OFF_F = TT_OFF_P + 2 * TT_PBUF;  // and their factors
 constexpr int TT_OFF_W = TT_OFF_F + 1024;         // o on its way out, 4 KB a warp
-constexpr int TT_OFF_QS = TT_OFF_VAL + 2 * TT_GRP * TT_M * 4;  // queries on their way in, 2 KB a warp
-constexpr int TT_SMEM_SCORE = TT_OFF_QS + 4 * TT_GRP * 2048;
+constexpr int TT_SMEM_SCORE = TT_OFF_VAL + 2 * TT_GRP * TT_M * 4;
 constexpr int TT_SMEM_VALUE = TT_OFF_W + 4 * TT_GRP * 4096;
 constexpr int TT_SMEM = (TT_SMEM_SCORE > TT_SMEM_VALUE ? TT_SMEM_SCORE : TT_SMEM_VALUE) + 1024;
 static_assert(TT_OFF_W % 1024 == 0 && 2 * TT_M * 4 <= 1024, "the stages are swizzled");
@@ -132,7 +131,7 @@ struct TreeArgs {
 };
 
 struct TreeMaps {
-    CUtensorMap lat_k, lat_v, rope;
+    CUtensorMap lat_k, lat_v, rope, q, q_rope;
 };
 
 // A cluster's next piece of the line: tiles t0 .. t1 - 1 of row tile mt of sequence b.
@@ -284,6 +283,7 @@ __global__ void __launch_bounds__(1024) mla_tree_plan(PagedView v, int H, TreePl
 struct TreeBars {
     uint64_t full[TT_KCH], empty[TT_KCH];  // stages
     uint64_t q_full, q_empty;              // score: queries in place; their last S is done
+    uint64_t q_read[TT_KCH];               // score: a stage of queries is taken
     uint64_t s_full[2], s_empty[2];        // score
     uint64_t pair[4];                      // score: per lane quarter, its two warps
     uint64_t p_out, p_ack;                 // score: P is written; the peer has it
@@ -312,7 +312,7 @@ __device__ __forceinline__ void rescale_o(uint32_t addr, int n, float f) {
 // row0: to the partial, or (a whole row tile) as the projection's bf16 hi/lo pair. A lane reads its
 // row from TMEM; the rows go through 4 KB of shared memory so that they are stored 64 or 128 bytes of
 // a row at a time (stored straight from the lanes, 16 bytes of 32 rows each, this took 20000 cycles).
-// Here and in load_q the loops stay rolled: what runs once per row tile is not in the instruction
+// Here and in take_q the loops stay rolled: what runs once per row tile is not in the instruction
 // cache, and every 128 bytes of it cost some 250 cycles.
 __device__ __forceinline__ void write_o(const TreeArgs &a, const TreeSeg &g, int cl, uint32_t addr,
                                         uint8_t *stage, int row0, int dim, int n) {
@@ -370,59 +370,47 @@ __device__ __forceinline__ void write_o(const TreeArgs &a, const TreeSeg &g, int
     }
 }
 
-// A row tile's queries: the latent dims into TMEM (lane = row, two bf16 per column), group grp of a
-// quarter one half of them; the rope dims into shared memory, 32 dims a group. Rows past the last
-// token's are zero. A negative scale is taken by the queries' sign, and a scale of zero makes them
-// zero. A warp reads 64 bytes of 8 rows at a time and turns them round in 2 KB of shared memory.
-__device__ __forceinline__ void load_q(const TreeArgs &a, const TreeSeg &g, uint32_t lane_addr,
-                                       uint8_t *stage, uint8_t *rope, int q4, int grp) {
-    const int lane = threadIdx.x & 31, r0 = 32 * q4, c = lane & 3;
-    const int rows = a.scale_log2e == 0.f ? 0 : min(32, g.s.n * a.H - (g.mt * TT_M + r0));
-    const uint32_t flip = a.scale_log2e < 0.f ? 0x80008000u : 0u;
-    const uint4 *q = reinterpret_cast<const uint4 *>(
-        a.qlat + ((size_t)g.s.first * a.H + g.mt * TT_M + r0 + (lane >> 2)) * TT_QW) + c;
-    // step k: 32 dims, the last the rope dims; rows 8 i + lane / 4, 16-byte chunk lane % 4
-    auto fetch = [&](uint4 (&w)[4], int k) {
-        const int dim = k < 8 ? 256 * grp + 32 * k : TT_DL + 32 * grp;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            w[i] = make_uint4(0, 0, 0, 0);
-            if (8 * i + (lane >> 2) < rows) {
-                const uint4 x = q[i * TT_QW + dim / 8];  // 8 rows of TT_QW / 8
-                w[i] = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
-            }
-        }
+// A row tile's queries, which the loads have put into the K stages (128 dims a stage, two 64-dim blocks
+// of 128 rows) and their rope dims into a buffer of their own: the latent dims into TMEM (lane = row,
+// two bf16 per column), group grp of a quarter one block of every stage. A negative scale is taken by
+// the queries' sign, and a scale of zero makes them zero. (Loads by the warps themselves, whatever
+// their order, took 13000 to 28000 cycles: global loads wait 3000 and more behind the TMA's.)
+__device__ __forceinline__ bool take_q(const TreeArgs &a, TreeBars &bars, uint8_t *sm,
+                                       uint32_t lane_addr, int row, int grp, int pass) {
+    const uint32_t keep = a.scale_log2e == 0.f ? 0u : ~0u, flip = a.scale_log2e < 0.f ? 0x80008000u : 0u;
+    auto fix = [&](uint4 x) {
+        return make_uint4((x.x & keep) ^ flip, (x.y & keep) ^ flip, (x.z & keep) ^ flip,
+                          (x.w & keep) ^ flip);
     };
-    auto at = [&](int r, int ch) { return stage + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4); };
-    uint4 w[4], next[4], after[4];
-    fetch(w, 0);
-    fetch(next, 1);
 #pragma unroll 1
-    for (int k = 0; k < 8; k++) {
-        fetch(after, k + 2 < 9 ? k + 2 : 8);
-        __syncwarp();
+    for (int c = 0; c < TT_KCH; c++) {
+        if (!warp_spin(&bars.full[c], pass & 1, a.err, 0x526)) return false;
+        const uint8_t *q = sm + c * TT_KSTAGE + grp * (TT_M * 128);
+        float v[32];
 #pragma unroll
-        for (int i = 0; i < 4; i++) st16s(at(8 * i + (lane >> 2), c), w[i]);
-        __syncwarp();
-        float v[16];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(at(lane, i));
+        for (int i = 0; i < 8; i++) {
+            const uint4 x = fix(*reinterpret_cast<const uint4 *>(q + swz(row, i)));
             v[4 * i] = __uint_as_float(x.x);
             v[4 * i + 1] = __uint_as_float(x.y);
             v[4 * i + 2] = __uint_as_float(x.z);
             v[4 * i + 3] = __uint_as_float(x.w);
         }
-        tmem_st16(lane_addr + TT_TM_Q + 128 * grp + 16 * k, v);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            w[i] = next[i];
-            next[i] = after[i];
+        if (c == 0 && (keep != ~0u || flip)) {
+#pragma unroll 1
+            for (int i = 4 * grp; i < 4 * grp + 4; i++) {
+                uint8_t *p = sm + TT_OFF_QR + swz(row, i);
+                st16s(p, fix(*reinterpret_cast<const uint4 *>(p)));
+            }
+            fence_async_shared();
         }
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(&bars.q_read[c]);
+        const uint32_t at = lane_addr + TT_TM_Q + 64 * c + 32 * grp;
+        tmem_st16(at, *reinterpret_cast<float(*)[16]>(v));
+        tmem_st16(at + 16, *reinterpret_cast<float(*)[16]>(v + 16));
     }
-#pragma unroll
-    for (int i = 0; i < 4; i++) st16s(rope + swz(r0 + 8 * i + (lane >> 2), 4 * grp + c), w[i]);
     tmem_wait_st();
+    return true;
 }
 
 // Zero what a draft row of bf16 pairs holds that is not finite.
@@ -441,7 +429,7 @@ __device__ __forceinline__ void tree_loads(const TreeMaps &maps, const TreeArgs 
     constexpr int STAGE = kScore ? TT_KSTAGE : TT_VSTAGE, RB = STAGE / ROWS;  // bytes of a row
     const int lane = threadIdx.x & 31;
     const int box = min(a.v.page_size, ROWS), per = ROWS / box;  // rows of a box, boxes of a chunk
-    int g = 0, loaded = 0;  // tiles; stages in use
+    int g = 0, nq = 0, loaded = 0;  // tiles; row tiles' queries; stages in use
     // this lane's box of a tile: its first cache row (page 0 where the table names no page)
     auto lookup = [&](const TreeSeg &sg, int t) -> int {
         const int p = t * TT_TILE + lane * box;
@@ -459,6 +447,24 @@ __device__ __forceinline__ void tree_loads(const TreeMaps &maps, const TreeArgs 
     for (; more && ok; g++) {
         const int live = (sg.s.len + sg.s.n - t * TT_TILE + box - 1) / box, at = row;
         if (!kScore && lane == 0) *(volatile int *)&bars.tile = g;
+        const bool fresh = kScore && t == sg.t0;  // a new row tile: its queries first
+        if (fresh) {
+            const int q0 = sg.s.first * a.H + sg.mt * TT_M;
+#pragma unroll 1
+            for (int c = 0; c < CH; c++) {
+                if (g > 0 && !(ok = warp_spin(&bars.empty[c], (g - 1) & 1, a.err, 0x503))) break;
+                if (lane == 0) {
+                    mbar_expect_tx(&bars.full[c], STAGE + (c == 0 ? TT_M * 128 : 0));
+                    tma_load_3d(sm + c * STAGE, &maps.q, &bars.full[c], 0, q0, 2 * c);
+                    if (c == 0)
+                        tma_load_2d(sm + TT_OFF_QR, &maps.q_rope, &bars.full[c], TT_DL, q0);
+                }
+                __syncwarp();
+                loaded = (loaded & ~(3 << (2 * c))) | (((g + nq) & 1 ? 2 : 1) << (2 * c));
+            }
+            if (!ok) break;
+            nq++;
+        }
         // the next tile's rows, looked up under this one's loads
         if (++t >= sg.t1) {
             more = walk.next(sg);
@@ -471,7 +477,9 @@ __device__ __forceinline__ void tree_loads(const TreeMaps &maps, const TreeArgs 
             const int first = kScore ? 0 : c * per, j = lane - first;
             const int n = max(0, min(per, live - first));
             const bool rope = kScore && c == 0;
-            if (g > 0 && !(ok = warp_spin(&bars.empty[c], (g - 1) & 1, a.err, 0x501))) break;
+            if (fresh) ok = warp_spin(&bars.q_read[c], (nq - 1) & 1, a.err, 0x504);
+            else if (g > 0) ok = warp_spin(&bars.empty[c], (g - 1) & 1, a.err, 0x501);
+            if (!ok) break;
             if (lane == 0) mbar_expect_tx(&bars.full[c], n * box * (RB + (rope ? 128 : 0)));
             __syncwarp();
             if (j >= 0 && j < n) {
@@ -480,7 +488,7 @@ __device__ __forceinline__ void tree_loads(const TreeMaps &maps, const TreeArgs 
                 if (rope)
                     tma_load_2d(sm + TT_OFF_KR + j * box * 128, &maps.rope, &bars.full[c], 0, at);
             }
-            loaded = (loaded & ~(3 << (2 * c))) | ((g & 1 ? 2 : 1) << (2 * c));
+            loaded = (loaded & ~(3 << (2 * c))) | (((g + nq) & 1 ? 2 : 1) << (2 * c));
         }
     }
     // loads still in flight are waited for (bounded) before the CTA may exit
@@ -520,6 +528,7 @@ __device__ __forceinline__ void score_mma(const TreeArgs &a, TreeWalk walk, uint
     TreeSeg sg;
     while (walk.next(sg)) {
         if (!warp_spin(&bars.q_full, nq++ & 1, a.err, 0x511)) return;
+        data = false;  // what was seen in advance were the queries
         for (int t = sg.t0; t < sg.t1; t++, g++) {
             const int sb = g & 1;
             const uint32_t d = tbase + TT_TM_S + sb * TT_TILE;
@@ -527,7 +536,7 @@ __device__ __forceinline__ void score_mma(const TreeArgs &a, TreeWalk walk, uint
             if (!room && !warp_spin(&bars.s_empty[sb], ((g >> 1) - 1) & 1, a.err, 0x512)) return;
 #pragma unroll 1
             for (int c = 0; c < TT_KCH; c++) {
-                if (!data && !warp_spin(&bars.full[c], g & 1, a.err, 0x513)) return;
+                if (!data && !warp_spin(&bars.full[c], (g + nq) & 1, a.err, 0x513)) return;
                 tc_fence_after();
                 uint64_t b = sdesc(smem_u32(sm + c * TT_KSTAGE), 16, 2048);
                 if (c == 0) {
@@ -540,9 +549,9 @@ __device__ __forceinline__ void score_mma(const TreeArgs &a, TreeWalk walk, uint
 #pragma unroll
                 for (int ks = 0; ks < 4; ks++) warp_mma_ts(d, q + ks * 8, b + ks * (32 >> 4), id, 1u);
                 if (c + 1 < TT_KCH) {
-                    data = __all_sync(0xffffffffu, mbar_test(&bars.full[c + 1], g & 1));
+                    data = __all_sync(0xffffffffu, mbar_test(&bars.full[c + 1], (g + nq) & 1));
                 } else {
-                    data = __all_sync(0xffffffffu, mbar_test(&bars.full[0], (g + 1) & 1));
+                    data = __all_sync(0xffffffffu, mbar_test(&bars.full[0], (g + nq + 1) & 1));
                     room = g < 1 || __all_sync(0xffffffffu, mbar_test(&bars.s_empty[sb ^ 1],
                                                                           (((g + 1) >> 1) - 1) & 1));
                 }
@@ -569,7 +578,7 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
     uint8_t *P = sm + TT_OFF_PS + grp * (TT_M * 128);  // this warp's 64-column block
     float *val = reinterpret_cast<float *>(sm + TT_OFF_VAL) + row;  // [2][TT_GRP][TT_M]
     // Scores are scaled to log2 units with the maximum's subtraction, by a positive factor (a masked
-    // -inf stays one): see load_q.
+    // -inf stays one): see take_q.
     const float scale = a.scale_log2e == 0.f ? 1.f : fabsf(a.scale_log2e);
     float m_ref = -INFINITY, l = 0.f;  // l: this warp's columns
     int g = 0, nq = 0, np = 0;
@@ -589,8 +598,7 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
         // this warp's part of the queries (the last row tile's S must be done)
         if (nq > 0 && !warp_spin(&bars.q_empty, (nq - 1) & 1, a.err, 0x522)) return;
         tc_fence_after();
-        load_q(a, sg, laddr, sm + TT_OFF_QS + (warp - 2) * 2048, sm + TT_OFF_QR, q4, grp);
-        fence_async_shared();
+        if (!take_q(a, bars, sm, laddr, row, grp, g + nq)) return;
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.q_full);
@@ -882,6 +890,7 @@ mla_tree_attend_tc(const __grid_constant__ TreeMaps maps, const __grid_constant_
             mbar_init(&bars.empty[c], 1);
         }
         for (int c = 0; c < TT_VCH; c++) mbar_init(&bars.clean[c], TT_WORKERS);
+        for (int c = 0; c < TT_KCH; c++) mbar_init(&bars.q_read[c], TT_WORKERS);
         mbar_init(&bars.q_full, TT_WORKERS);
         mbar_init(&bars.q_empty, 1);
         for (int q = 0; q < 4; q++) mbar_init(&bars.pair[q], TT_GRP);
@@ -1058,6 +1067,13 @@ extern "C" int k3cuda_mla_tree_attend(k3cuda_ctx *ctx, void *out, int out_dtype,
     if (!rc)
         rc = make_tmap_2d(&maps.rope, cache->rope, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, TT_DR, rows,
                           TT_DR * 2, 64, kbox);
+    const uint64_t qrows = (uint64_t)T * H;
+    if (!rc)
+        rc = make_tmap_3d(&maps.q, qlat, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 64, qrows, TT_DL / 64,
+                          TT_QW * 2, 128, 64, TT_M, 2);
+    if (!rc)
+        rc = make_tmap_2d(&maps.q_rope, qlat, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, TT_QW, qrows,
+                          TT_QW * 2, 64, TT_M);
     if (rc || (rc = set_smem(mla_tree_attend_tc, TT_SMEM))) return rc;
 
     int clusters = ctx->sm_count / 2;
