@@ -4,14 +4,17 @@
 //     log p_i = (x_i - m) - log s          entropy = log s - t / s
 // One pass over the logits: a thread keeps a running (m, s, t) and rescales s and t when m grows
 // (t' = f (t + s (m - m')), f = e^(m - m')). Sums are fp32; x - m is formed before it is scaled to
-// log2 units, so large logits lose nothing.
+// log2 units, so large logits lose nothing. Pairs of logits share an instruction (fp32 pairs; the
+// maximum of bf16 logits on bf16 pairs): 4.5 instructions a logit, of them one exponential, 16 a
+// clock and SM.
 //
 // The K likeliest tokens come out of the same pass. A thread writes the maximum of each group of
 // logits it reads (its cell) to shared memory. The K-th largest of some thread maxima is a bound
 // that at least K logits reach, so only cells that reach it are read again (from L2, a few dozen
-// of thousands), and the handful of logits at or above it are ranked by (logit, lower number).
-// Where more of them reach it than the buffer holds (rows of equal logits), the block instead
-// searches the row K times.
+// of thousands): they are listed first and read all at once, since one after another, as each
+// thread meets its own, they took 13 us of a block. The handful of logits at or above the bound
+// are ranked by (logit, lower number). Where more cells or logits reach it than the buffers hold
+// (rows of equal logits), the block instead searches the row K times.
 //
 // Rows are cut into segments of whole iterations when there are few of them: each block leaves
 // (m, s, t) and its K best, and a second kernel joins a row's segments.
@@ -22,10 +25,11 @@ namespace k3 {
 
 constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32;
 constexpr int LP_MAX_IT = 32;      // iterations of a segment (cells per thread)
-constexpr int LP_CAND = 1024;      // candidates ranked at once
+constexpr int LP_CAND = 1024;      // cells listed, candidates ranked at once
 constexpr int LP_MAX_SEG = 256;    // segments of a row
 constexpr int LP_MAX_V = 1 << 24;
 static_assert(K3CUDA_MAX_TOP * K3CUDA_MAX_TOP <= LP_CAND, "a join's candidates fit");
+static_assert(LP_MAX_IT * LP_THREADS <= 65536, "a cell's number has 16 bits");
 constexpr float LP_LOG2E = 1.4426950408889634f;
 
 typedef unsigned long long u64;
@@ -48,18 +52,16 @@ __device__ __forceinline__ u64 key_of(float x, int i) {
 struct Stat {
     float m, s, t;
 };
-__device__ __forceinline__ Stat join(Stat a, Stat b) {
-    Stat r;
-    r.m = fmaxf(a.m, b.m);
-    // an empty side (s = 0) has m = -inf; NaN sums stay NaN
-    const float da = a.m - r.m, db = b.m - r.m;
-    const float fa = a.s == 0.f ? 0.f : sm100::ex2_approx(da * LP_LOG2E);
-    const float fb = b.s == 0.f ? 0.f : sm100::ex2_approx(db * LP_LOG2E);
-    r.s = a.s * fa + b.s * fb;
-    r.t = 0.f;
-    if (a.s != 0.f) r.t += fa * (a.t + a.s * fmaxf(da, -1000.f));
-    if (b.s != 0.f) r.t += fb * (b.t + b.s * fmaxf(db, -1000.f));
-    return r;
+// (s, t) of a maximum m taken to a maximum M >= m
+__device__ __forceinline__ void move(Stat &a, float M) {
+    if (a.s == 0.f) {  // an empty set: m = -inf (NaN sums stay NaN)
+        a.t = 0.f;
+    } else {
+        const float d = a.m - M, f = sm100::ex2_approx(d * LP_LOG2E);
+        a.t = f * (a.t + a.s * fmaxf(d, -1000.f));
+        a.s *= f;
+    }
+    a.m = M;
 }
 
 struct LpArgs {
@@ -84,12 +86,52 @@ template <> struct vec<float> {
         x[0] = __uint_as_float(r.x); x[1] = __uint_as_float(r.y);
         x[2] = __uint_as_float(r.z); x[3] = __uint_as_float(r.w);
     }
+    // of U vectors, as of fmaxf: NaN is no maximum
+    template <int U> static __device__ __forceinline__ float max(const uint4 *r) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float x[N];
+            unpack(r[u], x);
+            m = sm100::max3(sm100::max3(m, x[0], x[1]), x[2], x[3]);
+        }
+        return m;
+    }
 };
 template <> struct vec<__nv_bfloat16> {
     static constexpr int N = 8;
     static constexpr unsigned NINF = 0xff80ff80u;
     static __device__ __forceinline__ void unpack(uint4 r, float *x) { sm100::unpack_bf8(r, x); }
+    template <int U> static __device__ __forceinline__ float max(const uint4 *r) {
+        __nv_bfloat162 m = reinterpret_cast<const __nv_bfloat162 &>(r[0].x);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const __nv_bfloat162 *x = reinterpret_cast<const __nv_bfloat162 *>(r + u);
+#pragma unroll
+            for (int i = u == 0; i < 4; i++) m = __hmax2(m, x[i]);
+        }
+        const float lo = __low2float(m), hi = __high2float(m);
+        return fmaxf(fmaxf(lo, hi), -INFINITY);  // -inf where all are NaN
+    }
 };
+
+// The vector of logits e .. of a row of V where some are outside of it: those are -inf.
+template <typename T> __device__ __noinline__ uint4 edge_load(const T *x, int e, int V) {
+    constexpr int N = vec<T>::N;
+    unsigned w[4] = {vec<T>::NINF, vec<T>::NINF, vec<T>::NINF, vec<T>::NINF};
+#pragma unroll
+    for (int j = 0; j < N; j++)
+        if (e + j >= 0 && e + j < V) {
+            if (sizeof(T) == 4) {
+                w[j & 3] = reinterpret_cast<const unsigned *>(x)[e + j];
+            } else {
+                const unsigned h = reinterpret_cast<const unsigned short *>(x)[e + j];
+                const int sh = 16 * (j & 1);
+                w[(j >> 1) & 3] = (w[(j >> 1) & 3] & ~(0xffffu << sh)) | (h << sh);
+            }
+        }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
 
 // A row as 16-byte vectors from the vector boundary at or before its first logit: vector v holds
 // logits v N - skew .. +N. The vectors at the row's ends are read logit by logit.
@@ -102,30 +144,20 @@ template <typename T> struct Row {
         skew = (int)(((uintptr_t)x / sizeof(T)) % vec<T>::N);
     }
     __device__ __forceinline__ int vectors() const { return (V + skew + vec<T>::N - 1) / vec<T>::N; }
+    // vectors lo .. hi - 1 are whole
+    __device__ __forceinline__ int lo() const { return skew > 0; }
+    __device__ __forceinline__ int hi() const { return (V + skew) / vec<T>::N; }
+    __device__ __forceinline__ uint4 whole(int v) const {
+        uint4 r;
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                     : "l"(x + ((long long)v * vec<T>::N - skew)));
+        return r;
+    }
     __device__ __forceinline__ uint4 load(int v, int end) const {
-        constexpr int N = vec<T>::N;
-        const int e = v * N - skew;
-        uint4 r = make_uint4(vec<T>::NINF, vec<T>::NINF, vec<T>::NINF, vec<T>::NINF);
-        if (v >= end) return r;
-        if (e >= 0 && e + N <= V) {
-            asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-                         : "l"(x + e));
-            return r;
-        }
-        unsigned w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int j = 0; j < N; j++)
-            if (e + j >= 0 && e + j < V) {
-                if (sizeof(T) == 4) {
-                    w[j & 3] = reinterpret_cast<const unsigned *>(x)[e + j];
-                } else {
-                    const unsigned h = reinterpret_cast<const unsigned short *>(x)[e + j];
-                    const int sh = 16 * (j & 1);
-                    w[(j >> 1) & 3] = (w[(j >> 1) & 3] & ~(0xffffu << sh)) | (h << sh);
-                }
-            }
-        return make_uint4(w[0], w[1], w[2], w[3]);
+        if (v >= lo() && v < min(hi(), end)) return whole(v);
+        if (v < end) return edge_load<T>(x, v * vec<T>::N - skew, V);
+        return make_uint4(vec<T>::NINF, vec<T>::NINF, vec<T>::NINF, vec<T>::NINF);
     }
 };
 
@@ -160,19 +192,31 @@ __device__ __forceinline__ void finish_row(const LpArgs &a, int row, Stat st, co
 
 // the block's joined statistics, in every thread
 __device__ __forceinline__ Stat block_join(Stat st, Stat *red) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // the maximum, as an ordered number; then plain sums
+    const float m = unord(__reduce_max_sync(0xffffffffu, ord(st.m)));
+    if (lane == 0) red[warp].m = m;
+    __syncthreads();
+    float M = red[0].m;
+#pragma unroll
+    for (int w = 1; w < LP_WARPS; w++) M = fmaxf(M, red[w].m);
+    move(st, M);
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
-        Stat b;
-        b.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-        b.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-        b.t = __shfl_xor_sync(0xffffffffu, st.t, o);
-        // the same order on both lanes of a pair, so that they agree bit for bit
-        st = (threadIdx.x & o) ? join(b, st) : join(st, b);
+        st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
+        st.t += __shfl_xor_sync(0xffffffffu, st.t, o);
     }
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = st;
+    if (lane == 0) {
+        red[warp].s = st.s;
+        red[warp].t = st.t;
+    }
     __syncthreads();
-    st = red[0];
-    for (int w = 1; w < LP_WARPS; w++) st = join(st, red[w]);
+    st.s = st.t = 0.f;
+#pragma unroll
+    for (int w = 0; w < LP_WARPS; w++) {
+        st.s += red[w].s;
+        st.t += red[w].t;
+    }
     return st;
 }
 
@@ -193,7 +237,8 @@ struct LpShared {
     Stat red[LP_WARPS];
     unsigned head[32];        // thread maxima that set the bound
     unsigned bound;
-    int n;
+    int n, cells;
+    unsigned short list[LP_CAND];  // cells that reach the bound
     u64 cand[LP_CAND], best[K3CUDA_MAX_TOP], wbest[LP_WARPS];
 };
 
@@ -226,6 +271,14 @@ __device__ __forceinline__ unsigned block_bound(float m, int K, LpShared &sh) {
     return sh.bound;
 }
 
+template <int U> __device__ __forceinline__ uint4 pick(const uint4 *r, int u) {
+    uint4 x = r[0];
+#pragma unroll
+    for (int i = 1; i < U; i++)
+        if (u == i) x = r[i];
+    return x;
+}
+
 // U: 16-byte vectors a thread reads per iteration
 template <typename T, int U>
 __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_k(const LpArgs a) {
@@ -240,62 +293,95 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_k(const LpArgs a
     const int v1 = min(r.vectors(), v0 + a.n_it * U * LP_THREADS);
     const int its = v1 > v0 ? (v1 - v0 + U * LP_THREADS - 1) / (U * LP_THREADS) : 0;
     Stat st{-INFINITY, 0.f, 0.f};
-    uint4 raw[U];
+    const int lo = r.lo(), hi = min(r.hi(), v1);
+    // iteration it's vectors (-inf behind the last)
+    auto fetch = [&](uint4 *raw, int it) {
+        const int v = v0 + it * U * LP_THREADS;
+        if (v >= lo && v + U * LP_THREADS <= hi) {
 #pragma unroll
-    for (int u = 0; u < U; u++) raw[u] = r.load(v0 + u * LP_THREADS + tid, v1);
-    for (int it = 0; it < its; it++) {
-        uint4 next[U];  // the next iteration's loads are in flight while this one is summed
-        const int vn = v0 + (it + 1) * U * LP_THREADS + tid;
+            for (int u = 0; u < U; u++) raw[u] = r.whole(v + tid + u * LP_THREADS);
+        } else {
 #pragma unroll
-        for (int u = 0; u < U; u++) next[u] = r.load(vn + u * LP_THREADS, v1);
-        float x[U * N];
-#pragma unroll
-        for (int u = 0; u < U; u++) vec<T>::unpack(raw[u], x + u * N);
-        float cm = x[0];
-#pragma unroll
-        for (int i = 1; i < U * N; i++) cm = fmaxf(cm, x[i]);
+            for (int u = 0; u < U; u++) raw[u] = r.load(v + tid + u * LP_THREADS, v1);
+        }
+    };
+    auto add = [&](const uint4 *raw, int it) {
+        const float cm = vec<T>::template max<U>(raw);
         if (a.K) cell[it * LP_THREADS + tid] = cm;
-        if (cm > st.m) {
-            const float d = st.m - cm, f = sm100::ex2_approx(d * LP_LOG2E);
-            st.t = st.s > 0.f ? f * (st.t + st.s * fmaxf(d, -1000.f)) : 0.f;
-            st.s *= f;
-            st.m = cm;
-        }
+        if (cm > st.m) move(st, cm);
         const float m = st.m == -INFINITY ? 0.f : st.m;
+        const float2 m2 = make_float2(-m, -m), k2 = make_float2(LP_LOG2E, LP_LOG2E);
+        float2 s2 = make_float2(0.f, 0.f), t2 = s2;
 #pragma unroll
-        for (int i = 0; i < U * N; i++) {
-            const float d = x[i] - m;
-            const float e = sm100::ex2_approx(d * LP_LOG2E);
-            st.s += e;
-            st.t = fmaf(e, fmaxf(d, -1000.f), st.t);
+        for (int u = 0; u < U; u++) {
+            float x[N];
+            vec<T>::unpack(raw[u], x);
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
+                const float2 d = sm100::add2(make_float2(x[i], x[i + 1]), m2);
+                float2 e = sm100::mul2(d, k2);
+                e.x = sm100::ex2_approx(e.x);
+                e.y = sm100::ex2_approx(e.y);
+                s2 = sm100::add2(s2, e);
+                t2 = sm100::fma2(e, d, t2);
+            }
         }
+        float t = t2.x + t2.y;
+        if (!(t == t)) {  // a forbidden token's 0 times -inf among them: without those
+            t = 0.f;
+#pragma unroll 1
+            for (int u = 0; u < U; u++) {
+                float x[N];
+                vec<T>::unpack(pick<U>(raw, u), x);
 #pragma unroll
-        for (int u = 0; u < U; u++) raw[u] = next[u];
+                for (int i = 0; i < N; i++) {
+                    const float d = x[i] - m;
+                    t = fmaf(sm100::ex2_approx(d * LP_LOG2E), fmaxf(d, -1000.f), t);
+                }
+            }
+        }
+        st.s += s2.x + s2.y;
+        st.t += t;
+    };
+    uint4 ra[U], rb[U];  // one iteration's loads are in flight while the other is summed
+    fetch(ra, 0);
+#pragma unroll 1
+    for (int it = 0; it < its; it += 2) {
+        fetch(rb, it + 1);
+        add(ra, it);
+        if (it + 1 >= its) break;
+        fetch(ra, it + 2);
+        add(rb, it + 1);
     }
     const float tm = st.m;
     const Stat all = block_join(st, sh.red);
     if (a.K) {
         const unsigned bound = block_bound(tm, a.K, sh);
-        if (tid == 0) sh.n = 0;
+        if (tid == 0) sh.n = sh.cells = 0;
         __syncthreads();
         if (ord(tm) >= bound)
             for (int it = 0; it < its; it++) {
                 if (ord(cell[it * LP_THREADS + tid]) < bound) continue;
-                for (int u = 0; u < U; u++) {
-                    const int v = v0 + (it * U + u) * LP_THREADS + tid;
-                    float x[N];
-                    vec<T>::unpack(r.load(v, v1), x);
-#pragma unroll
-                    for (int i = 0; i < N; i++)
-                        if (ord(x[i]) >= bound && x[i] <= INFINITY) {
-                            const int p = atomicAdd(&sh.n, 1);
-                            if (p < LP_CAND) sh.cand[p] = key_of(x[i], v * N - r.skew + i);
-                        }
-                }
+                const int p = atomicAdd(&sh.cells, 1);
+                if (p < LP_CAND) sh.list[p] = (unsigned short)(it * LP_THREADS + tid);
             }
         __syncthreads();
+        const int cells = sh.cells;
+        for (int e = tid; e < min(cells, LP_CAND) * U; e += LP_THREADS) {
+            const int c = sh.list[e / U];
+            const int v = v0 + (c / LP_THREADS * U + e % U) * LP_THREADS + c % LP_THREADS;
+            float x[N];
+            vec<T>::unpack(r.load(v, v1), x);
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if (ord(x[i]) >= bound && x[i] <= INFINITY) {
+                    const int p = atomicAdd(&sh.n, 1);
+                    if (p < LP_CAND) sh.cand[p] = key_of(x[i], v * N - r.skew + i);
+                }
+        }
+        __syncthreads();
         const int n = sh.n;
-        if (n <= LP_CAND) {
+        if (cells <= LP_CAND && n <= LP_CAND) {
             rank_keys(sh.cand, n, a.K, sh.best);
         } else {
             // the next best, K times
@@ -359,13 +445,13 @@ template <typename T> __global__ void __launch_bounds__(LP_THREADS) token_logpro
         __syncthreads();
         const u64 least = max(bound, 1ull);
         __syncthreads();
-        if (tid < a.S)
-            for (int k = 0; k < a.K; k++) {
-                const u64 key = keys[(size_t)tid * a.K + k];
-                if (key < least) break;
-                const int p = atomicAdd(&sh.n, 1);
-                if (p < LP_CAND) sh.cand[p] = key;
-            }
+#pragma unroll 4
+        for (int i = tid; i < a.S * a.K; i += LP_THREADS) {
+            const u64 key = keys[i];
+            if (key < least) continue;
+            const int p = atomicAdd(&sh.n, 1);
+            if (p < LP_CAND) sh.cand[p] = key;
+        }
         __syncthreads();
         rank_keys(sh.cand, min(sh.n, LP_CAND), a.K, sh.best);
     }

@@ -499,27 +499,6 @@ __device__ __forceinline__ void tree_loads(const TreeMaps &maps, const TreeArgs 
 }
 
 // ---------------------------------------------------------------- score CTA
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(reinterpret_cast<uint64_t &>(d))
-        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)),
-          "l"(reinterpret_cast<uint64_t &>(c)));
-    return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("add.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<uint64_t &>(d))
-        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
-    return d;
-}
-
 __device__ __forceinline__ void score_mma(const TreeArgs &a, TreeWalk walk, uint8_t *sm,
                                           TreeBars &bars, uint32_t tbase) {
     constexpr uint32_t id = idesc_f16(128, TT_TILE, false, false);
