@@ -161,20 +161,25 @@ template <typename T> struct Row {
     }
 };
 
-// What a row's statistics and K best give: the outputs (block-wide; keys in shared memory, 0 for
-// a place without a token).
+// the logit of a row's g-th given token, -inf without one
 template <typename T>
-__device__ __forceinline__ void finish_row(const LpArgs &a, int row, Stat st, const u64 *best) {
-    const T *x = static_cast<const T *>(a.logits) + (size_t)row * a.stride;
+__device__ __forceinline__ float given(const LpArgs &a, int row, int g) {
+    const int tok = g < a.G ? a.tokens[(size_t)row * a.G + g] : -1;
+    if (tok < 0 || tok >= a.V) return -INFINITY;
+    return io<T>::ld(static_cast<const T *>(a.logits) + (size_t)row * a.stride + tok);
+}
+
+// What a row's statistics and K best give: the outputs (block-wide; keys in shared memory, 0 for
+// a place without a token; mine: this thread's first given token's logit).
+template <typename T>
+__device__ __forceinline__ void finish_row(const LpArgs &a, int row, Stat st, float mine,
+                                           const u64 *best) {
     // no distribution: nothing but -inf (m = -inf), or a NaN or +inf (s is NaN then)
     const bool none = !(st.s > 0.f);
     const float ls = none ? NAN : logf(st.s);
     for (int g = threadIdx.x; g < a.G; g += LP_THREADS) {
-        const int tok = a.tokens[(size_t)row * a.G + g];
-        float lp = -INFINITY;
-        if (none) lp = NAN;
-        else if (tok >= 0 && tok < a.V) lp = (io<T>::ld(x + tok) - st.m) - ls;
-        a.logprobs[(size_t)row * a.G + g] = lp;
+        const float x = g == threadIdx.x ? mine : given<T>(a, row, g);
+        a.logprobs[(size_t)row * a.G + g] = none ? NAN : (x - st.m) - ls;
     }
     if (threadIdx.x == 0 && a.entropy) a.entropy[row] = none ? NAN : ls - st.t / st.s;
     for (int k = threadIdx.x; k < a.K; k += LP_THREADS) {
@@ -227,6 +232,7 @@ __device__ __forceinline__ void rank_keys(const u64 *cand, int n, int K, u64 *be
     for (int i = threadIdx.x; i < n; i += LP_THREADS) {
         const u64 mine = cand[i];
         int r = 0;
+#pragma unroll 4
         for (int j = 0; j < n; j++) r += cand[j] > mine;
         if (r < K) best[r] = mine;
     }
@@ -235,40 +241,22 @@ __device__ __forceinline__ void rank_keys(const u64 *cand, int n, int K, u64 *be
 
 struct LpShared {
     Stat red[LP_WARPS];
-    unsigned head[32];        // thread maxima that set the bound
-    unsigned bound;
     int n, cells;
     unsigned short list[LP_CAND];  // cells that reach the bound
     u64 cand[LP_CAND], best[K3CUDA_MAX_TOP], wbest[LP_WARPS];
 };
 
 // The bound: at least K logits of the block are at or above it (LP_ORD_NINF + 1 where fewer than
-// K are above -inf). Every warp gives its ceil(K / 8) largest thread maxima; the bound is the
-// K-th largest of those.
-__device__ __forceinline__ unsigned block_bound(float m, int K, LpShared &sh) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int per = (K + LP_WARPS - 1) / LP_WARPS;
-    unsigned mine = m == -INFINITY ? 0u : ord(m);
-    for (int j = 0; j < per; j++) {
-        const unsigned top = __reduce_max_sync(0xffffffffu, mine);
-        const unsigned has = __ballot_sync(0xffffffffu, mine == top);
-        if (lane == __ffs(has) - 1) mine = 0;
-        if (lane == 0) sh.head[warp * per + j] = top;
-    }
-    __syncthreads();
-    if (warp == 0) {
-        const int n = per * LP_WARPS;
-        const unsigned h = lane < n ? sh.head[lane] : 0u;
-        int r = 0;
-#pragma unroll
-        for (int j = 0; j < 32; j++) {
-            const unsigned o = __shfl_sync(0xffffffffu, h, j);
-            r += o > h || (o == h && j < lane);
-        }
-        if (r == K - 1) sh.bound = max(h, LP_ORD_NINF + 1);
-    }
-    __syncthreads();
-    return sh.bound;
+// K threads hold one above -inf). It is the K-th largest thread maximum to its upper 16 bits, found
+// bit by bit. (The K-th largest of every warp's ceil(K / 8) best is had sooner, but where a few warps
+// hold nothing but -inf there are too few of those, and all the others' logits were ranked: 7 us.)
+__device__ __forceinline__ unsigned block_bound(float m, int K) {
+    const unsigned mine = m == -INFINITY ? 0u : ord(m) >> 16;
+    unsigned at = 0;
+#pragma unroll 1
+    for (unsigned bit = 1u << 15; bit; bit >>= 1)
+        if (__syncthreads_count(mine >= (at | bit)) >= K) at |= bit;
+    return max(at << 16, LP_ORD_NINF + 1);
 }
 
 template <int U> __device__ __forceinline__ uint4 pick(const uint4 *r, int u) {
@@ -356,7 +344,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_k(const LpArgs a
     const float tm = st.m;
     const Stat all = block_join(st, sh.red);
     if (a.K) {
-        const unsigned bound = block_bound(tm, a.K, sh);
+        const unsigned bound = block_bound(tm, a.K);
         if (tid == 0) sh.n = sh.cells = 0;
         __syncthreads();
         if (ord(tm) >= bound)
@@ -367,17 +355,16 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_k(const LpArgs a
             }
         __syncthreads();
         const int cells = sh.cells;
-        for (int e = tid; e < min(cells, LP_CAND) * U; e += LP_THREADS) {
-            const int c = sh.list[e / U];
-            const int v = v0 + (c / LP_THREADS * U + e % U) * LP_THREADS + c % LP_THREADS;
-            float x[N];
-            vec<T>::unpack(r.load(v, v1), x);
-#pragma unroll
-            for (int i = 0; i < N; i++)
-                if (ord(x[i]) >= bound && x[i] <= INFINITY) {
-                    const int p = atomicAdd(&sh.n, 1);
-                    if (p < LP_CAND) sh.cand[p] = key_of(x[i], v * N - r.skew + i);
-                }
+#pragma unroll 1
+        for (int e = tid; e < min(cells, LP_CAND) * U * N; e += LP_THREADS) {
+            const int c = sh.list[e / (U * N)];
+            const int v = v0 + (c / LP_THREADS * U + e / N % U) * LP_THREADS + c % LP_THREADS;
+            const int i = v * N - r.skew + e % N;
+            if (v >= v1 || i < 0 || i >= r.V) continue;
+            const float x = io<T>::ld(r.x + i);
+            if (ord(x) < bound || !(x <= INFINITY)) continue;
+            const int p = atomicAdd(&sh.n, 1);
+            if (p < LP_CAND) sh.cand[p] = key_of(x, i);
         }
         __syncthreads();
         const int n = sh.n;
@@ -391,7 +378,6 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_k(const LpArgs a
                 for (int v = v0 + tid; v < v1; v += LP_THREADS) {
                     float x[N];
                     vec<T>::unpack(r.load(v, v1), x);
-#pragma unroll
                     for (int i = 0; i < N; i++) {
                         const u64 key = key_of(x[i], v * N - r.skew + i);
                         if (x[i] > -INFINITY && key < last && key > top) top = key;
@@ -410,7 +396,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_k(const LpArgs a
         }
     }
     if (a.S == 1) {
-        finish_row<T>(a, row, all, sh.best);
+        finish_row<T>(a, row, all, given<T>(a, row, tid), sh.best);
         return;
     }
     if (tid == 0) a.stats[blockIdx.x] = all;
@@ -429,6 +415,7 @@ template <typename T> __global__ void __launch_bounds__(LP_THREADS) token_logpro
     const u64 *keys = a.keys + (size_t)row * a.S * a.K;
     Stat st{-INFINITY, 0.f, 0.f};
     if (tid < a.S) st = ss[tid];
+    const float mine = given<T>(a, row, tid);  // on its way while the segments are joined
     const Stat all = block_join(st, sh.red);
     if (a.K) {
         const int per = (a.K + a.S - 1) / a.S, n = per * a.S;  // n < S + K <= LP_CAND
@@ -439,6 +426,7 @@ template <typename T> __global__ void __launch_bounds__(LP_THREADS) token_logpro
         for (int i = tid; i < n; i += LP_THREADS) {
             const u64 mine = sh.cand[i];
             int r = 0;
+#pragma unroll 4
             for (int j = 0; j < n; j++) r += sh.cand[j] > mine || (sh.cand[j] == mine && j < i);
             if (r == a.K - 1) bound = mine;  // 0 where fewer than K places hold a token
         }
@@ -455,7 +443,7 @@ template <typename T> __global__ void __launch_bounds__(LP_THREADS) token_logpro
         __syncthreads();
         rank_keys(sh.cand, min(sh.n, LP_CAND), a.K, sh.best);
     }
-    finish_row<T>(a, row, all, sh.best);
+    finish_row<T>(a, row, all, mine, sh.best);
 }
 
 // How rows are cut: U vectors per thread and iteration, n_it iterations per segment, S segments.
@@ -463,12 +451,12 @@ struct LpPlan {
     int U, n_it, S;
 };
 
-// Enough blocks to fill the GPU several times over where the rows allow it, on a B200's 148 SMs
+// Blocks to fill the GPU once (four an SM) where the rows allow it, on a B200's 148 SMs
 // whatever the device, so that the workspace query needs no device.
 static LpPlan lp_plan(int T, int V, int io_dtype) {
     const int N = io_dtype == K3CUDA_F32 ? 4 : 8;
     const long long nv = ((long long)V + 2 * N - 2) / N;  // most vectors, whatever the skew
-    constexpr long long want = 148 * 8;
+    constexpr long long want = 148 * 4;
     LpPlan p;
     p.U = T * ((nv + 4 * LP_THREADS - 1) / (4 * LP_THREADS)) >= want ? 4 : 1;
     const long long its = (nv + p.U * LP_THREADS - 1) / (p.U * LP_THREADS);
