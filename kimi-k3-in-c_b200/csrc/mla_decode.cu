@@ -124,19 +124,24 @@ mla_q_absorb_tc(const __grid_constant__ HeadGemmMaps maps, const __nv_bfloat16 *
         mbar_init(&bar_ld, 1);
         mbar_init(&bar_mma, 1);
         fence_barrier_init();
+        mbar_expect_tx(&bar_ld, 2 * 16384 + 8 * 8192);
+        // the weights are never written by the chain; q_nope is
+        for (int kb = 0; kb < 2; kb++)
+            for (int nb = 0; nb < 4; nb++)
+                tma_load_3d(sB + (kb * 4 + nb) * 8192, &maps.b, &bar_ld, (4 * z + nb) * 64, kb * 64,
+                            h);
     }
+    // The next kernel may start once every CTA is past the wait: what came before is done then.
+    // TMEM is taken after it too, so that no CTA holds any while an earlier kernel may want some.
+    pdl_wait();
+    pdl_trigger();
     if (warp == 1) tmem_alloc(&tslot, 256);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tb = tslot;
     if (tid == 0) {
-        mbar_expect_tx(&bar_ld, 2 * 16384 + 8 * 8192);
         for (int kb = 0; kb < 2; kb++) tma_load_3d(sA + kb * 16384, &maps.a, &bar_ld, kb * 64, h, b0);
-        for (int kb = 0; kb < 2; kb++)
-            for (int nb = 0; nb < 4; nb++)
-                tma_load_3d(sB + (kb * 4 + nb) * 8192, &maps.b, &bar_ld, (4 * z + nb) * 64, kb * 64,
-                            h);
         if (mbar_wait(&bar_ld, 0, err, 0x401)) {
             tc_fence_after();
             constexpr uint32_t id = idesc_f16(128, 256, false, true);
@@ -231,19 +236,25 @@ mla_project_tc(const __grid_constant__ HeadGemmMaps maps, OUT *__restrict__ out,
         }
         fence_barrier_init();
     }
+    // block kb into stage kb % NS: the weights (never written by the chain), and o_lat
+    auto load_w = [&](int kb) {
+        mbar_expect_tx(&bar_full[kb % NS], STAGE);
+        tma_load_3d(sm + (kb % NS) * STAGE + 16384, &maps.b, &bar_full[kb % NS], (kb % 8) * 64, 0, h);
+    };
+    auto load_o = [&](int kb) {
+        tma_load_3d(sm + (kb % NS) * STAGE, &maps.a, &bar_full[kb % NS], kb * 64, h, b0);
+    };
+    if (tid == 0)
+        for (int kb = 0; kb < NS; kb++) load_w(kb);
+    pdl_wait();  // TMEM is taken after the wait, as in mla_q_absorb_tc
+    pdl_trigger();
     if (warp == 1) tmem_alloc(&tslot, 128);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tb = tslot;
     if (tid == 0) {
-        auto load = [&](int kb) {  // block kb into stage kb % NS
-            uint8_t *st = sm + (kb % NS) * STAGE;
-            mbar_expect_tx(&bar_full[kb % NS], STAGE);
-            tma_load_3d(st, &maps.a, &bar_full[kb % NS], kb * 64, h, b0);
-            tma_load_3d(st + 16384, &maps.b, &bar_full[kb % NS], (kb % 8) * 64, 0, h);
-        };
-        for (int kb = 0; kb < NS; kb++) load(kb);
+        for (int kb = 0; kb < NS; kb++) load_o(kb);
         bool ok = true;
         constexpr uint32_t id = idesc_f16(128, 128, false, false);
         for (int kb = 0; kb < KB && ok; kb++) {
@@ -260,7 +271,8 @@ mla_project_tc(const __grid_constant__ HeadGemmMaps maps, OUT *__restrict__ out,
             const int pk = kb - 1;
             if (pk >= 0 && pk + NS < KB) {
                 if (!(ok = mbar_wait(&bar_empty[pk % NS], (pk / NS) & 1, err, 0x413))) break;
-                load(pk + NS);
+                load_w(pk + NS);
+                load_o(pk + NS);
             }
         }
         if (ok) mma_commit(&bar_mma);
@@ -708,7 +720,6 @@ mla_q_absorb_small(const __nv_bfloat16 *__restrict__ q_nope,
                    long long uk_head_elems, __nv_bfloat16 *__restrict__ qlat, int pitch, int B, int H) {
     __shared__ float qs[NB][MLA_DN];
     __shared__ float red[8][NB][128];
-    pdl_trigger();
     const int h = blockIdx.x, z = blockIdx.y, tid = threadIdx.x, warp = tid >> 5;
     const int cg = tid & 15, r0 = tid >> 4, c0 = 128 * z + 8 * cg;
     uint4 wv[8];
@@ -719,6 +730,7 @@ mla_q_absorb_small(const __nv_bfloat16 *__restrict__ q_nope,
             wv[j] = __ldg(reinterpret_cast<const uint4 *>(W + (size_t)(r0 + 16 * j) * MLA_DL));
     }
     pdl_wait();  // the weights above are never written by the chain; q_nope is
+    pdl_trigger();  // what came before is done when the next kernel starts
     if (h >= H) {
         // a padding head of the MMA's M: its query row must score zero
         for (int e = tid; e < B * 128; e += 256)
@@ -1053,8 +1065,8 @@ int mla_absorb(k3cuda_ctx *ctx, __nv_bfloat16 *qlat, int pitch, const void *q_no
     const int smem = 2 * 16384 + 8 * 8192 + 1024;
     if ((rc = set_smem(mla_q_absorb_tc, smem))) return rc;
     const dim3 grid(H, (B + 127) / 128, 2);  // two 256-column halves of q_lat per head
-    mla_q_absorb_tc<<<grid, 128, smem, ctx->stream>>>(maps, qr, qlat, pitch, B, H, ctx->err_word);
-    return after_launch(ctx, "mla_q_absorb_tc");
+    return launch_pdl(ctx, ctx->stream, "mla_q_absorb_tc", mla_q_absorb_tc, grid, dim3(128), smem,
+                      maps, qr, qlat, pitch, B, H, ctx->err_word);
 }
 
 // out[b][h] = W_UV[h] o_lat[b][h] / rowsum[b][h], o_lat as bf16 hi/lo pairs [B][H][2 MLA_DL];
@@ -1084,16 +1096,15 @@ int mla_project(k3cuda_ctx *ctx, void *out, int out_dtype, const __nv_bfloat16 *
     if (rc) return rc;
     const dim3 grid(H, (B + 127) / 128);
     const int smem = 3 * 2 * 16384 + 1024;
+    const char *nm = "mla_project_tc";
     if (bf) {
         if ((rc = set_smem(mla_project_tc<__nv_bfloat16>, smem))) return rc;
-        mla_project_tc<__nv_bfloat16><<<grid, 128, smem, ctx->stream>>>(
-            maps, (__nv_bfloat16 *)out, B, H, rowsum, keep, ctx->err_word);
-    } else {
-        if ((rc = set_smem(mla_project_tc<float>, smem))) return rc;
-        mla_project_tc<float><<<grid, 128, smem, ctx->stream>>>(maps, (float *)out, B, H, rowsum,
-                                                                keep, ctx->err_word);
+        return launch_pdl(ctx, ctx->stream, nm, mla_project_tc<__nv_bfloat16>, grid, dim3(128), smem,
+                          maps, (__nv_bfloat16 *)out, B, H, rowsum, keep, ctx->err_word);
     }
-    return after_launch(ctx, "mla_project_tc");
+    if ((rc = set_smem(mla_project_tc<float>, smem))) return rc;
+    return launch_pdl(ctx, ctx->stream, nm, mla_project_tc<float>, grid, dim3(128), smem, maps,
+                      (float *)out, B, H, rowsum, keep, ctx->err_word);
 }
 
 }  // namespace k3

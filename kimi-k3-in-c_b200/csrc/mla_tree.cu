@@ -188,12 +188,13 @@ struct TreeWalk {
 };
 
 // Plan: the line's prefix over the sequences, which tokens count, and what is wrong with the tables.
+// It runs beside mla_absorb, whose CTAs let it start once what came before is done, and waits for that
+// kernel at its end, so that the attention waits for both.
 __global__ void __launch_bounds__(1024) mla_tree_plan(PagedView v, int H, TreePlan *plan,
                                                       long long *cum, int *keep, int clusters,
                                                       unsigned *err) {
     __shared__ long long wsum[32], carry, tsum[32];
     pdl_trigger();
-    pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     for (int t = tid; t < v.T; t += 1024) keep[t] = 0;
     if (tid == 0) carry = 0;
@@ -278,6 +279,7 @@ __global__ void __launch_bounds__(1024) mla_tree_plan(PagedView v, int H, TreePl
         if (cut[tid].last >= 0) plan->cut[at++] = cut[tid];
         if (tid + 1 == TT_CLUSTERS) plan->cuts = at;
     }
+    pdl_wait();
 }
 
 struct TreeBars {
@@ -886,13 +888,14 @@ mla_tree_attend_tc(const __grid_constant__ TreeMaps maps, const __grid_constant_
         fence_barrier_init();
         prefetch_tmap(score ? &maps.lat_k : &maps.lat_v);
     }
+    __syncthreads();
+    cluster_sync();  // the peer's barriers are ready before anything arrives on them
+    pdl_wait();      // the plan, the queries and the cache come from earlier work
     if (warp == 1) tmem_alloc(&bars.tmem_base, TT_TM_COLS);
     tc_fence_before();
     __syncthreads();
-    cluster_sync();  // the peer's barriers are ready before anything arrives on them
     tc_fence_after();
     const uint32_t tbase = bars.tmem_base;
-    pdl_wait();  // the plan, the queries and the cache come from earlier work
     const int G = a.plan->G;
     if (cl < G) tree_roles(maps, a, TreeWalk(a, cl, a.plan->total, G), sm, bars, tbase, cl, score);
     tc_fence_before();
@@ -901,58 +904,68 @@ mla_tree_attend_tc(const __grid_constant__ TreeMaps maps, const __grid_constant_
     if (warp == 1) tmem_dealloc(tbase, TT_TM_COLS);
 }
 
-// Join the row tiles that several clusters took (the flash-decoding identity), a row per block and
-// round; thread t owns latent dims 4 t .. 4 t + 3.
-__global__ void __launch_bounds__(128) mla_tree_join(const __grid_constant__ TreeArgs a) {
+// Join the row tiles that several clusters took (the flash-decoding identity), a row per warp and
+// round: the lanes take the parts' (m, l) first, then float4s lane, lane + 32, .. of every part.
+// Bound by L2's latency: with a row per block of 128 threads it took 16 us for 73 cut tiles, and two
+// rounds of rows take the place of eight now.
+constexpr int TJ_WARPS = 4;
+__global__ void __launch_bounds__(TJ_WARPS * 32, 8) mla_tree_join(const __grid_constant__ TreeArgs a) {
     pdl_trigger();
     pdl_wait();
-    const int tid = threadIdx.x, items = a.plan->cuts * TT_M;
+    const int lane = threadIdx.x & 31, items = a.plan->cuts * TT_M;
     const size_t stride = (size_t)2 * TT_M * TT_PART;  // between clusters
-    for (int i = blockIdx.x; i < items; i += gridDim.x) {
+    for (int i = blockIdx.x * TJ_WARPS + (threadIdx.x >> 5); i < items; i += gridDim.x * TJ_WARPS) {
         const TreeCut cut = a.plan->cut[i / TT_M];
         const int row = i % TT_M, c = cut.first;
         if (row >= cut.rows) continue;
         const float *base = a.part + (size_t)row * TT_PART;
         auto part = [&](int k) { return base + k * stride + (k == c ? TT_M * TT_PART : 0); };
         float M = -INFINITY;
-        for (int k = c; k <= cut.last; k++) M = fmaxf(M, part(k)[TT_DL]);
-        float L = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k0 = c; k0 <= cut.last; k0 += 4) {
-            float4 v[4];
-            float w[4], pl[4];
+        for (int k = c + lane; k <= cut.last; k += 32) M = fmaxf(M, part(k)[TT_DL]);
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                w[u] = pl[u] = 0.f;
-                v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (k0 + u <= cut.last) {
-                    const float *p = part(k0 + u);
-                    const float m = p[TT_DL];
-                    pl[u] = p[TT_DL + 1];
-                    w[u] = m == -INFINITY && pl[u] == 0.f ? 0.f : exp2f(m - M);
-                    v[u] = reinterpret_cast<const float4 *>(p)[tid];
+        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        float L = 0.f, o[4][4] = {};
+        for (int k0 = c; k0 <= cut.last; k0 += 32) {
+            float w = 0.f, pl = 0.f;
+            if (k0 + lane <= cut.last) {
+                const float *p = part(k0 + lane);
+                const float m = p[TT_DL];
+                pl = p[TT_DL + 1];
+                w = m == -INFINITY && pl == 0.f ? 0.f : exp2f(m - M);
+            }
+            pl *= w;
+#pragma unroll
+            for (int s = 16; s; s >>= 1) pl += __shfl_xor_sync(0xffffffffu, pl, s);
+            L += pl;
+            const int n = min(32, cut.last + 1 - k0);
+#pragma unroll 2
+            for (int k = 0; k < n; k++) {
+                const float4 *p = reinterpret_cast<const float4 *>(part(k0 + k)) + lane;
+                const float wk = __shfl_sync(0xffffffffu, w, k);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float4 v = p[32 * j];
+                    o[j][0] = fmaf(wk, v.x, o[j][0]);
+                    o[j][1] = fmaf(wk, v.y, o[j][1]);
+                    o[j][2] = fmaf(wk, v.z, o[j][2]);
+                    o[j][3] = fmaf(wk, v.w, o[j][3]);
                 }
             }
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                L += w[u] * pl[u];
-                o.x += w[u] * v[u].x;
-                o.y += w[u] * v[u].y;
-                o.z += w[u] * v[u].z;
-                o.w += w[u] * v[u].w;
-            }
         }
-        const float ov[4] = {o.x, o.y, o.z, o.w};
-        float lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) lo[i] = ov[i] - __bfloat162float(__float2bfloat16_rn(ov[i]));
         const size_t th = (size_t)cut.row0 + row;
         __nv_bfloat16 *dst = a.olat2 + th * 2 * TT_DL;
-        reinterpret_cast<uint2 *>(dst)[tid] =
-            make_uint2(pack_bf2(ov[0], ov[1]), pack_bf2(ov[2], ov[3]));
-        reinterpret_cast<uint2 *>(dst + TT_DL)[tid] =
-            make_uint2(pack_bf2(lo[0], lo[1]), pack_bf2(lo[2], lo[3]));
-        if (tid == 0) a.rowsum[th] = L;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                lo[e] = o[j][e] - __bfloat162float(__float2bfloat16_rn(o[j][e]));
+            reinterpret_cast<uint2 *>(dst)[lane + 32 * j] =
+                make_uint2(pack_bf2(o[j][0], o[j][1]), pack_bf2(o[j][2], o[j][3]));
+            reinterpret_cast<uint2 *>(dst + TT_DL)[lane + 32 * j] =
+                make_uint2(pack_bf2(lo[0], lo[1]), pack_bf2(lo[2], lo[3]));
+        }
+        if (lane == 0) a.rowsum[th] = L;
     }
 }
 
@@ -1058,15 +1071,16 @@ extern "C" int k3cuda_mla_tree_attend(k3cuda_ctx *ctx, void *out, int out_dtype,
     int clusters = ctx->sm_count / 2;
     if (clusters > TT_CLUSTERS) clusters = TT_CLUSTERS;
     if (clusters < 1) clusters = 1;
-    rc = launch_pdl(ctx, ctx->stream, "mla_tree_plan", mla_tree_plan, dim3(1), dim3(1024), 0, a.v, H,
-                    plan, cum, keep, clusters, ctx->err_word);
-    if (!rc) rc = mla_absorb(ctx, qlat, H, q_nope, q_rope, w_uk, TT_DN, T, H);
+    rc = mla_absorb(ctx, qlat, H, q_nope, q_rope, w_uk, TT_DN, T, H);
+    if (!rc)
+        rc = launch_pdl(ctx, ctx->stream, "mla_tree_plan", mla_tree_plan, dim3(1), dim3(1024), 0, a.v,
+                        H, plan, cum, keep, clusters, ctx->err_word);
     if (!rc)
         rc = launch_pdl(ctx, ctx->stream, "mla_tree_attend_tc", mla_tree_attend_tc,
                         dim3(2 * clusters), dim3(TT_THREADS), TT_SMEM, maps, a);
     if (!rc)
         rc = launch_pdl(ctx, ctx->stream, "mla_tree_join", mla_tree_join, dim3(8 * ctx->sm_count),
-                        dim3(128), 0, a);
+                        dim3(TJ_WARPS * 32), 0, a);
     if (!rc)
         rc = mla_project(ctx, out, out_dtype, a.olat2, a.rowsum, keep, w_uv, TT_DV, T, H);
     return rc;
