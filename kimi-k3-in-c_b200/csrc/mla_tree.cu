@@ -284,8 +284,6 @@ __global__ void __launch_bounds__(1024) mla_tree_plan(PagedView v, int H, TreePl
 
 struct TreeBars {
     uint64_t full[TT_KCH], empty[TT_KCH];  // stages
-    uint64_t q_full, q_empty;              // score: queries in place; their last S is done
-    uint64_t q_read[TT_KCH];               // score: a stage of queries is taken
     uint64_t s_full[2], s_empty[2];        // score
     uint64_t pair[4];                      // score: per lane quarter, its two warps
     uint64_t p_out, p_ack;                 // score: P is written; the peer has it
@@ -314,8 +312,8 @@ __device__ __forceinline__ void rescale_o(uint32_t addr, int n, float f) {
 // row0: to the partial, or (a whole row tile) as the projection's bf16 hi/lo pair. A lane reads its
 // row from TMEM; the rows go through 4 KB of shared memory so that they are stored 64 or 128 bytes of
 // a row at a time (stored straight from the lanes, 16 bytes of 32 rows each, this took 20000 cycles).
-// Here and in take_q the loops stay rolled: what runs once per row tile is not in the instruction
-// cache, and every 128 bytes of it cost some 250 cycles.
+// The loops stay rolled: what runs once per row tile is not in the instruction cache, and every 128
+// bytes of it cost some 250 cycles.
 __device__ __forceinline__ void write_o(const TreeArgs &a, const TreeSeg &g, int cl, uint32_t addr,
                                         uint8_t *stage, int row0, int dim, int n) {
     const int lane = threadIdx.x & 31, j = lane & 7;
@@ -372,49 +370,6 @@ __device__ __forceinline__ void write_o(const TreeArgs &a, const TreeSeg &g, int
     }
 }
 
-// A row tile's queries, which the loads have put into the K stages (128 dims a stage, two 64-dim blocks
-// of 128 rows) and their rope dims into a buffer of their own: the latent dims into TMEM (lane = row,
-// two bf16 per column), group grp of a quarter one block of every stage. A negative scale is taken by
-// the queries' sign, and a scale of zero makes them zero. (Loads by the warps themselves, whatever
-// their order, took 13000 to 28000 cycles: global loads wait 3000 and more behind the TMA's.)
-__device__ __forceinline__ bool take_q(const TreeArgs &a, TreeBars &bars, uint8_t *sm,
-                                       uint32_t lane_addr, int row, int grp, int pass) {
-    const uint32_t keep = a.scale_log2e == 0.f ? 0u : ~0u, flip = a.scale_log2e < 0.f ? 0x80008000u : 0u;
-    auto fix = [&](uint4 x) {
-        return make_uint4((x.x & keep) ^ flip, (x.y & keep) ^ flip, (x.z & keep) ^ flip,
-                          (x.w & keep) ^ flip);
-    };
-#pragma unroll 1
-    for (int c = 0; c < TT_KCH; c++) {
-        if (!warp_spin(&bars.full[c], pass & 1, a.err, 0x526)) return false;
-        const uint8_t *q = sm + c * TT_KSTAGE + grp * (TT_M * 128);
-        float v[32];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint4 x = fix(*reinterpret_cast<const uint4 *>(q + swz(row, i)));
-            v[4 * i] = __uint_as_float(x.x);
-            v[4 * i + 1] = __uint_as_float(x.y);
-            v[4 * i + 2] = __uint_as_float(x.z);
-            v[4 * i + 3] = __uint_as_float(x.w);
-        }
-        if (c == 0 && (keep != ~0u || flip)) {
-#pragma unroll 1
-            for (int i = 4 * grp; i < 4 * grp + 4; i++) {
-                uint8_t *p = sm + TT_OFF_QR + swz(row, i);
-                st16s(p, fix(*reinterpret_cast<const uint4 *>(p)));
-            }
-            fence_async_shared();
-        }
-        __syncwarp();
-        if ((threadIdx.x & 31) == 0) mbar_arrive(&bars.q_read[c]);
-        const uint32_t at = lane_addr + TT_TM_Q + 64 * c + 32 * grp;
-        tmem_st16(at, *reinterpret_cast<float(*)[16]>(v));
-        tmem_st16(at + 16, *reinterpret_cast<float(*)[16]>(v + 16));
-    }
-    tmem_wait_st();
-    return true;
-}
-
 // Zero what a draft row of bf16 pairs holds that is not finite.
 __device__ __forceinline__ uint32_t finite_pair(uint32_t u) {
     if ((u & 0x7f80u) == 0x7f80u) u &= 0xffff0000u;
@@ -423,7 +378,8 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t u) {
 }
 
 // A CTA's loads, chunk by chunk: for the score CTA 128 rows x 128 latent dims, the rope dims with
-// the first; for the value CTA 64 rows x 512 dims. Chunk c of every tile is in stage c.
+// the first; for the value CTA 32 rows x 512 dims. Chunk c of every tile is in stage c. In the score
+// CTA a row tile's queries come through the same stages before its first tile.
 template <bool kScore>
 __device__ __forceinline__ void tree_loads(const TreeMaps &maps, const TreeArgs &a, TreeWalk walk,
                                            uint8_t *sm, TreeBars &bars) {
@@ -431,7 +387,7 @@ __device__ __forceinline__ void tree_loads(const TreeMaps &maps, const TreeArgs 
     constexpr int STAGE = kScore ? TT_KSTAGE : TT_VSTAGE, RB = STAGE / ROWS;  // bytes of a row
     const int lane = threadIdx.x & 31;
     const int box = min(a.v.page_size, ROWS), per = ROWS / box;  // rows of a box, boxes of a chunk
-    int g = 0, nq = 0, loaded = 0;  // tiles; row tiles' queries; stages in use
+    int k = 0, loaded = 0;  // times the stages were filled; which of them, and in which phase
     // this lane's box of a tile: its first cache row (page 0 where the table names no page)
     auto lookup = [&](const TreeSeg &sg, int t) -> int {
         const int p = t * TT_TILE + lane * box;
@@ -443,18 +399,18 @@ __device__ __forceinline__ void tree_loads(const TreeMaps &maps, const TreeArgs 
         }
         return (int)r;
     };
+    auto free = [&](int c) { return k == 0 || warp_spin(&bars.empty[c], (k - 1) & 1, a.err, 0x501); };
+    auto used = [&](int c) { loaded = (loaded & ~(3 << (2 * c))) | ((k & 1 ? 2 : 1) << (2 * c)); };
     TreeSeg sg;
     bool more = walk.next(sg), ok = true;
     int t = more ? sg.t0 : 0, row = more ? lookup(sg, t) : 0;
-    for (; more && ok; g++) {
+    for (; more && ok; k++) {
         const int live = (sg.s.len + sg.s.n - t * TT_TILE + box - 1) / box, at = row;
-        if (!kScore && lane == 0) *(volatile int *)&bars.tile = g;
-        const bool fresh = kScore && t == sg.t0;  // a new row tile: its queries first
-        if (fresh) {
+        if (!kScore && lane == 0) *(volatile int *)&bars.tile = k;
+        if (kScore && t == sg.t0) {
             const int q0 = sg.s.first * a.H + sg.mt * TT_M;
 #pragma unroll 1
-            for (int c = 0; c < CH; c++) {
-                if (g > 0 && !(ok = warp_spin(&bars.empty[c], (g - 1) & 1, a.err, 0x503))) break;
+            for (int c = 0; c < CH && (ok = free(c)); c++) {
                 if (lane == 0) {
                     mbar_expect_tx(&bars.full[c], STAGE + (c == 0 ? TT_M * 128 : 0));
                     tma_load_3d(sm + c * STAGE, &maps.q, &bars.full[c], 0, q0, 2 * c);
@@ -462,10 +418,10 @@ __device__ __forceinline__ void tree_loads(const TreeMaps &maps, const TreeArgs 
                         tma_load_2d(sm + TT_OFF_QR, &maps.q_rope, &bars.full[c], TT_DL, q0);
                 }
                 __syncwarp();
-                loaded = (loaded & ~(3 << (2 * c))) | (((g + nq) & 1 ? 2 : 1) << (2 * c));
+                used(c);
             }
             if (!ok) break;
-            nq++;
+            k++;
         }
         // the next tile's rows, looked up under this one's loads
         if (++t >= sg.t1) {
@@ -474,14 +430,11 @@ __device__ __forceinline__ void tree_loads(const TreeMaps &maps, const TreeArgs 
         }
         if (more) row = lookup(sg, t);
 #pragma unroll 1
-        for (int c = 0; c < CH; c++) {
+        for (int c = 0; c < CH && (ok = free(c)); c++) {
             // the lanes whose boxes this chunk takes: all of them, or those of its rows
             const int first = kScore ? 0 : c * per, j = lane - first;
             const int n = max(0, min(per, live - first));
             const bool rope = kScore && c == 0;
-            if (fresh) ok = warp_spin(&bars.q_read[c], (nq - 1) & 1, a.err, 0x504);
-            else if (g > 0) ok = warp_spin(&bars.empty[c], (g - 1) & 1, a.err, 0x501);
-            if (!ok) break;
             if (lane == 0) mbar_expect_tx(&bars.full[c], n * box * (RB + (rope ? 128 : 0)));
             __syncwarp();
             if (j >= 0 && j < n) {
@@ -490,7 +443,7 @@ __device__ __forceinline__ void tree_loads(const TreeMaps &maps, const TreeArgs 
                 if (rope)
                     tma_load_2d(sm + TT_OFF_KR + j * box * 128, &maps.rope, &bars.full[c], 0, at);
             }
-            loaded = (loaded & ~(3 << (2 * c))) | (((g + nq) & 1 ? 2 : 1) << (2 * c));
+            used(c);
         }
     }
     // loads still in flight are waited for (bounded) before the CTA may exit
@@ -504,20 +457,36 @@ __device__ __forceinline__ void tree_loads(const TreeMaps &maps, const TreeArgs 
 __device__ __forceinline__ void score_mma(const TreeArgs &a, TreeWalk walk, uint8_t *sm,
                                           TreeBars &bars, uint32_t tbase) {
     constexpr uint32_t id = idesc_f16(128, TT_TILE, false, false);
-    int g = 0, nq = 0;
+    int g = 0, k = 0;                // tiles; fillings of the stages (tiles and queries)
     bool data = false, room = true;  // the next chunk and score buffer, as seen in advance
     TreeSeg sg;
     while (walk.next(sg)) {
-        if (!warp_spin(&bars.q_full, nq++ & 1, a.err, 0x511)) return;
-        data = false;  // what was seen in advance were the queries
-        for (int t = sg.t0; t < sg.t1; t++, g++) {
+        // The queries into TMEM, 16 dims at a time, once the last row tile's scores are formed. (Taken
+        // there by the softmax warps, a row tile's first scores came 5000 cycles later.)
+        if (g > 0 && !warp_spin(&bars.s_full[(g - 1) & 1], ((g - 1) >> 1) & 1, a.err, 0x511)) return;
+#pragma unroll 1
+        for (int c = 0; c < TT_KCH; c++) {
+            if (!data && !warp_spin(&bars.full[c], k & 1, a.err, 0x514)) return;
+            tc_fence_after();
+            uint64_t q = sdesc_kmajor(smem_u32(sm + c * TT_KSTAGE));
+            uint32_t d = tbase + TT_TM_Q + 64 * c;
+#pragma unroll 1
+            for (int half = 0; half < 2; half++, q += (TT_M * 128) >> 4, d += 32) {
+#pragma unroll
+                for (int ks = 0; ks < 4; ks++) warp_copy(d + ks * 8, q + ks * (32 >> 4));
+            }
+            warp_commit(&bars.empty[c]);
+            data = false;
+        }
+        k++;
+        for (int t = sg.t0; t < sg.t1; t++, g++, k++) {
             const int sb = g & 1;
             const uint32_t d = tbase + TT_TM_S + sb * TT_TILE;
             uint32_t q = tbase + TT_TM_Q;
             if (!room && !warp_spin(&bars.s_empty[sb], ((g >> 1) - 1) & 1, a.err, 0x512)) return;
 #pragma unroll 1
             for (int c = 0; c < TT_KCH; c++) {
-                if (!data && !warp_spin(&bars.full[c], (g + nq) & 1, a.err, 0x513)) return;
+                if (!data && !warp_spin(&bars.full[c], k & 1, a.err, 0x513)) return;
                 tc_fence_after();
                 uint64_t b = sdesc(smem_u32(sm + c * TT_KSTAGE), 16, 2048);
                 if (c == 0) {
@@ -530,9 +499,9 @@ __device__ __forceinline__ void score_mma(const TreeArgs &a, TreeWalk walk, uint
 #pragma unroll
                 for (int ks = 0; ks < 4; ks++) warp_mma_ts(d, q + ks * 8, b + ks * (32 >> 4), id, 1u);
                 if (c + 1 < TT_KCH) {
-                    data = __all_sync(0xffffffffu, mbar_test(&bars.full[c + 1], (g + nq) & 1));
+                    data = __all_sync(0xffffffffu, mbar_test(&bars.full[c + 1], k & 1));
                 } else {
-                    data = __all_sync(0xffffffffu, mbar_test(&bars.full[0], (g + nq + 1) & 1));
+                    data = __all_sync(0xffffffffu, mbar_test(&bars.full[0], (k + 1) & 1));
                     room = g < 1 || __all_sync(0xffffffffu, mbar_test(&bars.s_empty[sb ^ 1],
                                                                           (((g + 1) >> 1) - 1) & 1));
                 }
@@ -544,7 +513,6 @@ __device__ __forceinline__ void score_mma(const TreeArgs &a, TreeWalk walk, uint
                 if (c + 1 == TT_KCH) warp_commit(&bars.s_full[sb]);
                 warp_commit(&bars.empty[c]);
             }
-            if (t + 1 == sg.t1) warp_commit(&bars.q_empty);
         }
     }
 }
@@ -558,11 +526,12 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
     const uint32_t laddr = tbase + ((uint32_t)(32 * q4) << 16);
     uint8_t *P = sm + TT_OFF_PS + grp * (TT_M * 128);  // this warp's 64-column block
     float *val = reinterpret_cast<float *>(sm + TT_OFF_VAL) + row;  // [2][TT_GRP][TT_M]
-    // Scores are scaled to log2 units with the maximum's subtraction, by a positive factor (a masked
-    // -inf stays one): see take_q.
+    // Scores are scaled to log2 units with the maximum's subtraction, by a positive factor, so that a
+    // masked -inf stays one; the sign of a negative scale, or a scale of zero, is taken before.
+    const float sign = a.scale_log2e > 0.f ? 1.f : a.scale_log2e < 0.f ? -1.f : 0.f;
     const float scale = a.scale_log2e == 0.f ? 1.f : fabsf(a.scale_log2e);
     float m_ref = -INFINITY, l = 0.f;  // l: this warp's columns
-    int g = 0, nq = 0, np = 0;
+    int g = 0, np = 0;
     // the other warp's value of the row
     auto share = [&](float v, float &o) -> bool {
         float *at = val + (np & 1) * TT_GRP * TT_M;
@@ -576,14 +545,6 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
     };
     TreeSeg sg;
     while (walk.next(sg)) {
-        // this warp's part of the queries (the last row tile's S must be done)
-        if (nq > 0 && !warp_spin(&bars.q_empty, (nq - 1) & 1, a.err, 0x522)) return;
-        tc_fence_after();
-        if (!take_q(a, bars, sm, laddr, row, grp, g + nq)) return;
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.q_full);
-        nq++;
         // the word of this row's token
         const int tok = min((sg.mt * TT_M + row) / a.H, sg.s.n - 1);
         const uint64_t word = a.mask ? a.mask[sg.s.first + tok] : (((uint64_t)2 << tok) - 1);
@@ -593,7 +554,7 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
             if (!warp_spin(&bars.s_full[sb], (g >> 1) & 1, a.err, 0x523)) return;
             tc_fence_after();
             const int p0 = t * TT_TILE + c0;
-            if (p0 + TT_CW > sg.s.len) {  // reaches past the cached rows: masked in TMEM
+            if (p0 + TT_CW > sg.s.len || sign != 1.f) {  // past the cached rows: masked in TMEM
                 const uint64_t see = tree_bits(word, sg.s.len, sg.s.n, p0);
                 const int d0 = sg.s.len - p0;
 #pragma unroll 1
@@ -603,6 +564,7 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
                     tmem_wait_ld();
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
+                        x[i] *= sign;
                         if (c + i >= d0 && !(fabsf(x[i]) < INFINITY)) x[i] = NAN;
                         if (!((see >> (c + i)) & 1)) x[i] = -INFINITY;
                     }
@@ -712,20 +674,25 @@ __device__ __forceinline__ void value_mma(const TreeArgs &a, TreeWalk walk, uint
         for (int t = sg.t0; t < sg.t1; t++, g++) {
             const int pb = g & 1;
             const bool edge = (long long)(t + 1) * TT_TILE > sg.s.len;
+            const int live = min(TT_TILE, sg.s.len + sg.s.n - t * TT_TILE);  // rows of the tile
             if (!ready && !warp_spin(&bars.p_full[pb], (g >> 1) & 1, a.err, 0x541)) return;
 #pragma unroll 1
             for (int c = 0; c < TT_VCH; c++) {
                 if (!data && !warp_spin(&bars.full[c], g & 1, a.err, 0x542)) return;
-                if (edge && !warp_spin(&bars.clean[c], edges & 1, a.err, 0x543)) return;
+                if (edge && c * TT_VROWS < live && !warp_spin(&bars.clean[c], edges & 1, a.err, 0x543))
+                    return;
                 tc_fence_after();
                 // 16 rows at a time: P's columns, the rows' 512 dims in two halves
                 const uint64_t kv = sdesc(smem_u32(sm + c * TT_VSTAGE), 1024, 8192);
                 const uint64_t pd = sdesc_kmajor(
                     smem_u32(sm + TT_OFF_P + pb * TT_PBUF + (c >> 1) * TT_M * 128 + (c & 1) * 64));
                 const uint32_t acc = (t == sg.t0 && c == 0) ? 0u : 1u;
-                warp_mma_ss(tbase, pd, kv, id, acc);
-                warp_mma_ss(tbase + 256, pd, kv + (4096 >> 4), id, acc);
-                warp_mma_ss(tbase, pd + (32 >> 4), kv + (16384 >> 4), id, 1u);
+                const bool some = c * TT_VROWS < live;  // else its weights are all zero
+                if (some) {
+                    warp_mma_ss(tbase, pd, kv, id, acc);
+                    warp_mma_ss(tbase + 256, pd, kv + (4096 >> 4), id, acc);
+                    warp_mma_ss(tbase, pd + (32 >> 4), kv + (16384 >> 4), id, 1u);
+                }
                 if (c + 1 < TT_VCH) {
                     data = __all_sync(0xffffffffu, mbar_test(&bars.full[c + 1], g & 1));
                 } else {
@@ -733,7 +700,7 @@ __device__ __forceinline__ void value_mma(const TreeArgs &a, TreeWalk walk, uint
                     ready = __all_sync(0xffffffffu,
                                        mbar_test(&bars.p_full[pb ^ 1], ((g + 1) >> 1) & 1));
                 }
-                warp_mma_ss(tbase + 256, pd + (32 >> 4), kv + (20480 >> 4), id, 1u);
+                if (some) warp_mma_ss(tbase + 256, pd + (32 >> 4), kv + (20480 >> 4), id, 1u);
                 if (c + 1 == TT_VCH) warp_commit_cluster(&bars.pv_done[pb], 3);
                 warp_commit(&bars.empty[c]);
             }
@@ -804,27 +771,32 @@ __device__ __forceinline__ void value_output(const TreeArgs &a, TreeWalk walk, u
             if (lane == 0) mbar_arrive(&bars.p_full[pb]);
             if ((long long)(t + 1) * TT_TILE <= sg.s.len) continue;
             // rows past the cached ones: zero where nothing is written, and where a draft's element
-            // is not finite
+            // is not finite (a chunk without rows is left out of the products)
+            const int live = sg.s.len + sg.s.n - t * TT_TILE;
+#pragma unroll 1
             for (int c = 0; c < TT_VCH; c++) {
-                if (!warp_spin(&bars.full[c], g & 1, a.err, 0x554)) return;
-                const long long d0 = sg.s.len - ((long long)t * TT_TILE + c * TT_VROWS);
-                const long long d1 = d0 + sg.s.n;
-                uint8_t *kv = sm + c * TT_VSTAGE;
-                for (int e = threadIdx.x - 64; e < TT_VROWS * 64; e += TT_WORKERS * 32) {
-                    const int r = e / 64, kb = (e / 8) % 8, ch = e % 8;
-                    if (r < d0) continue;
-                    uint4 *p = reinterpret_cast<uint4 *>(kv + (r / 8) * 8192 + kb * 1024 +
-                                                         (r % 8) * 128 + ch * 16);
-                    uint4 w = make_uint4(0, 0, 0, 0);
-                    if (r < d1) {
-                        w = *p;
-                        w = make_uint4(finite_pair(w.x), finite_pair(w.y), finite_pair(w.z),
-                                       finite_pair(w.w));
+                if (c * TT_VROWS < live) {
+                    if (!warp_spin(&bars.full[c], g & 1, a.err, 0x554)) return;
+                    const int d0 = max(0, sg.s.len - (t * TT_TILE + c * TT_VROWS));
+                    const int d1 = live - c * TT_VROWS;
+                    // a warp per row; a lane's 16 bytes of two 64-dim blocks
+#pragma unroll 1
+                    for (int e = 2 * d0 + warp - 2; e < 2 * TT_VROWS; e += TT_WORKERS) {
+                        const int r = e / 2;
+                        uint4 *p = reinterpret_cast<uint4 *>(
+                            sm + c * TT_VSTAGE + (r / 8) * 8192 + (4 * (e & 1) + lane / 8) * 1024 +
+                            (r % 8) * 128 + (lane % 8) * 16);
+                        uint4 w = make_uint4(0, 0, 0, 0);
+                        if (r < d1) {
+                            w = *p;
+                            w = make_uint4(finite_pair(w.x), finite_pair(w.y), finite_pair(w.z),
+                                           finite_pair(w.w));
+                        }
+                        *p = w;
                     }
-                    *p = w;
+                    fence_async_shared();
+                    __syncwarp();
                 }
-                fence_async_shared();
-                __syncwarp();
                 if (lane == 0) mbar_arrive(&bars.clean[c]);
             }
         }
@@ -871,9 +843,6 @@ mla_tree_attend_tc(const __grid_constant__ TreeMaps maps, const __grid_constant_
             mbar_init(&bars.empty[c], 1);
         }
         for (int c = 0; c < TT_VCH; c++) mbar_init(&bars.clean[c], TT_WORKERS);
-        for (int c = 0; c < TT_KCH; c++) mbar_init(&bars.q_read[c], TT_WORKERS);
-        mbar_init(&bars.q_full, TT_WORKERS);
-        mbar_init(&bars.q_empty, 1);
         for (int q = 0; q < 4; q++) mbar_init(&bars.pair[q], TT_GRP);
         mbar_init(&bars.p_out, TT_WORKERS);
         mbar_init(&bars.p_ack, 1);

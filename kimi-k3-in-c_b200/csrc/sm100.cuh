@@ -505,6 +505,15 @@ __device__ __forceinline__ void warp_mma_ss(uint32_t d_tmem, uint64_t adesc, uin
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// 128 rows x 32 bytes from shared memory to 8 TMEM columns; the warp's later MMAs come after it.
+__device__ __forceinline__ void warp_copy(uint32_t d_tmem, uint64_t desc) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.cp.cta_group::1.128x256b [%0], %1;\n\t}" ::"r"(d_tmem),
+        "l"(desc)
+        : "memory");
+}
 __device__ __forceinline__ void warp_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
                                             uint32_t idesc, uint32_t accumulate) {
     asm volatile(
