@@ -42,8 +42,8 @@
 // the score CTA's are busy half the time: sixteen softmax warps of 32 columns each slowed the loads
 // and the MMA issue by more than they gained.
 //
-// Work: the (row tile, cache tile) pairs lie on a line, every row tile taking TT_FIXED more places
-// for its fixed work; clusters take equal pieces (paged.cuh). A row tile that one cluster does
+// Work: the (row tile, cache tile) pairs lie on a line, every row tile taking some more places for
+// its fixed work; clusters take equal pieces (paged.cuh). A row tile that one cluster does
 // whole is written as (o, l); one that is cut leaves partial (m, l, o) that mla_tree_join joins.
 // The line is formed on the device from the batch's tables (mla_tree_plan), so that a captured
 // call follows them.
@@ -70,6 +70,7 @@ constexpr int TT_KSTAGE = TT_TILE * TT_DL * 2 / TT_KCH;
 constexpr int TT_VROWS = TT_TILE / TT_VCH;
 constexpr int TT_VSTAGE = TT_VROWS * TT_DL * 2;
 constexpr int TT_AHEAD = 4;                // tiles that rows are brought into L2 before their load
+constexpr int TT_PACE = 1600;              // ns between the first of them
 constexpr int TT_PBUF = 2 * TT_M * 128;    // two blocks of 64 columns
 constexpr int TT_OFF_KR = TT_KCH * TT_KSTAGE;     // score: rope dims of the tile
 constexpr int TT_OFF_QR = TT_OFF_KR + TT_TILE * 128;  // and of the query
@@ -92,8 +93,8 @@ constexpr int TT_WORKERS = 4 * TT_GRP;     // warps 2 ..
 constexpr int TT_THREADS = (3 + TT_WORKERS) * 32;
 constexpr int TT_CLUSTERS = 74;            // 148 SMs of a B200
 constexpr int TT_FIXED = 4;                // a row tile's fixed work, in tiles
-constexpr int TT_MIN_TILES = 2;            // fewest tiles per cluster
-constexpr int TT_PART = TT_DL + 4;         // floats of a partial row: o, m, l, pad
+// a partial, in floats: o [dims / 4][rows][4], m [rows], l [rows]
+constexpr int TT_PART_M = TT_DL * TT_M, TT_PART_L = TT_PART_M + TT_M, TT_PART = TT_PART_L + TT_M;
 // A row tile that is cut: the clusters with the first and the last part of it, its rows, and its first
 // row among all (token, head) rows.
 struct TreeCut {
@@ -111,6 +112,7 @@ struct TreeStart {
 struct TreePlan {
     long long total;   // places on the line
     int G;             // clusters that take part
+    int fixed;         // places of a row tile's fixed work
     int cuts;
     TreeCut cut[TT_CLUSTERS];
     TreeStart start[TT_CLUSTERS];
@@ -122,7 +124,7 @@ struct TreeArgs {
     const unsigned long long *mask;
     const __nv_bfloat16 *latent, *rope;  // the cache's rows
     const __nv_bfloat16 *qlat; // [T][H][576]
-    float *part;               // [2 TT_CLUSTERS][128][TT_PART]
+    float *part;               // [2 TT_CLUSTERS][TT_PART]
     __nv_bfloat16 *olat2;      // [T][H][hi 512 | lo 512]
     float *rowsum;             // [T][H]
     int H;
@@ -147,17 +149,18 @@ struct TreeSeg {
 struct TreeWalk {
     const TreeArgs &a;
     long long c0, c1, at;  // this cluster's places; the next row tile's first place
-    int b, mt, units;
+    int b, mt, units, fixed;
     long long cost;
     PagedSeq s;
     __device__ __forceinline__ void seq() {
         s = paged_seq(a.v, b, K3CUDA_MAX_DRAFTS);
         units = (int)(((long long)s.n * a.H + TT_M - 1) / TT_M);
-        cost = TT_FIXED + (s.len + s.n + TT_TILE - 1) / TT_TILE;
+        cost = fixed + (s.len + s.n + TT_TILE - 1) / TT_TILE;
     }
     __device__ __forceinline__ TreeWalk(const TreeArgs &args, int c, long long total, int G)
         : a(args), c0(line_begin(total, G, c)), c1(line_begin(total, G, c + 1)) {
         const TreeStart first = a.plan->start[c];
+        fixed = a.plan->fixed;
         b = first.b;
         mt = first.mt;
         at = first.at;
@@ -171,12 +174,12 @@ struct TreeWalk {
                 seq();
                 continue;
             }
-            const long long first = at + TT_FIXED;  // place of tile 0
+            const long long first = at + fixed;  // place of tile 0
             g.b = b;
             g.mt = mt;
             g.s = s;
             g.ustart = at;
-            g.tiles = (int)(cost - TT_FIXED);
+            g.tiles = (int)(cost - fixed);
             g.t0 = (int)(c0 > first ? c0 - first : 0);
             g.t1 = (int)(c1 < first ? 0 : c1 - first < g.tiles ? c1 - first : g.tiles);
             at += cost;
@@ -193,24 +196,35 @@ struct TreeWalk {
 __global__ void __launch_bounds__(1024) mla_tree_plan(PagedView v, int H, TreePlan *plan,
                                                       long long *cum, int *keep, int clusters,
                                                       unsigned *err) {
-    __shared__ long long wsum[32], carry, tsum[32];
+    __shared__ long long wsum[32], carry, all;
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     for (int t = tid; t < v.T; t += 1024) keep[t] = 0;
-    if (tid == 0) carry = 0;
+    if (tid == 0) carry = all = 0;
     __syncthreads();
-    long long tiles_all = 0;
+    long long tiles = 0;
+    for (int b = tid; b < v.B; b += 1024) {
+        const PagedSeq s = paged_seq(v, b, K3CUDA_MAX_DRAFTS);
+        if (s.code) atomicCAS(err + 1, 0u, (unsigned)s.code);
+        tiles += ((long long)s.n * H + TT_M - 1) / TT_M * ((s.len + s.n + TT_TILE - 1) / TT_TILE);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    if (lane == 0) atomicAdd((unsigned long long *)&all, (unsigned long long)tiles);
+    __syncthreads();
+    // A cluster has one tile at least. With no more than that for each, a row tile's fixed work is
+    // left out of account, or the clusters that its places fall to would have no tile.
+    tiles = all;
+    const int G = (int)(tiles < clusters ? tiles : clusters);
+    const int fixed = tiles > clusters ? TT_FIXED : 0;
     for (int b0 = 0; b0 < v.B; b0 += 1024) {
         const int b = b0 + tid;
         long long cost = 0;
         if (b < v.B) {
             const PagedSeq s = paged_seq(v, b, K3CUDA_MAX_DRAFTS);
-            if (s.code) atomicCAS(err + 1, 0u, (unsigned)s.code);
             for (int i = 0; i < s.n; i++) keep[s.first + i] = 1;
             const long long units = ((long long)s.n * H + TT_M - 1) / TT_M;
-            const long long tiles = (s.len + s.n + TT_TILE - 1) / TT_TILE;
-            cost = units * (tiles + TT_FIXED);
-            tiles_all += units * tiles;
+            cost = units * (fixed + (s.len + s.n + TT_TILE - 1) / TT_TILE);
         }
         long long x = cost;  // inclusive prefix over the block
 #pragma unroll
@@ -227,28 +241,21 @@ __global__ void __launch_bounds__(1024) mla_tree_plan(PagedView v, int H, TreePl
         if (tid == 1023) carry = before + x;
         __syncthreads();
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) tiles_all += __shfl_xor_sync(0xffffffffu, tiles_all, o);
-    if (lane == 0) tsum[warp] = tiles_all;
-    __syncthreads();
     if (tid == 0) {
-        long long tiles = 0;
-        for (int w = 0; w < 32; w++) tiles += tsum[w];
-        const long long want = (tiles + TT_MIN_TILES - 1) / TT_MIN_TILES;
         cum[v.B] = carry;
         plan->total = carry;
-        plan->G = (int)(want < clusters ? want : clusters);
+        plan->G = G;
+        plan->fixed = fixed;
     }
     __syncthreads();
-    // the row tile that holds each cluster's last place
-    const int G = plan->G;
+    // the row tile that holds each cluster's first place
     const long long total = carry;
     if (tid < G) {
         TreeStart start;
         const long long c0 = line_begin(total, G, tid);
         start.b = last_at_most(cum, v.B, c0);
         const PagedSeq s = paged_seq(v, start.b, K3CUDA_MAX_DRAFTS);
-        const long long cost = TT_FIXED + (s.len + s.n + TT_TILE - 1) / TT_TILE;
+        const long long cost = fixed + (s.len + s.n + TT_TILE - 1) / TT_TILE;
         start.mt = (int)((c0 - cum[start.b]) / cost);
         start.at = cum[start.b] + start.mt * cost;
         plan->start[tid] = start;
@@ -260,9 +267,9 @@ __global__ void __launch_bounds__(1024) mla_tree_plan(PagedView v, int H, TreePl
             const long long end = line_begin(total, G, tid + 1);
             const int b = last_at_most(cum, v.B, end - 1);
             const PagedSeq s = paged_seq(v, b, K3CUDA_MAX_DRAFTS);
-            const long long cost = TT_FIXED + (s.len + s.n + TT_TILE - 1) / TT_TILE;
+            const long long cost = fixed + (s.len + s.n + TT_TILE - 1) / TT_TILE;
             const int mt = (int)((end - 1 - cum[b]) / cost);
-            const long long first = cum[b] + mt * cost + TT_FIXED, last = first + cost - TT_FIXED - 1;
+            const long long first = cum[b] + mt * cost + fixed, last = first + cost - fixed - 1;
             // some of its tiles are in this cluster, the first among them, and some are not
             if (first < end && end <= last && first >= line_begin(total, G, tid)) {
                 cut[tid].first = tid;
@@ -309,59 +316,55 @@ __device__ __forceinline__ void rescale_o(uint32_t addr, int n, float f) {
 }
 
 // A segment's o, latent dims dim .. dim + n - 1 (TMEM columns from addr) of the warp's 32 rows from
-// row0: to the partial, or (a whole row tile) as the projection's bf16 hi/lo pair. A lane reads its
-// row from TMEM; the rows go through 4 KB of shared memory so that they are stored 64 or 128 bytes of
-// a row at a time (stored straight from the lanes, 16 bytes of 32 rows each, this took 20000 cycles).
+// row0. A lane reads its row from TMEM. A partial is laid out for that: 16 bytes of 32 rows follow one
+// another. A whole row tile goes out as the projection's bf16 hi/lo pair, through 4 KB of shared memory,
+// so that 64 bytes of a row are stored at a time (stored from the lanes, 16 bytes of 32 rows each, this
+// took 20000 cycles; through shared memory 11000; a partial 3000).
 // The loops stay rolled: what runs once per row tile is not in the instruction cache, and every 128
 // bytes of it cost some 250 cycles.
 __device__ __forceinline__ void write_o(const TreeArgs &a, const TreeSeg &g, int cl, uint32_t addr,
                                         uint8_t *stage, int row0, int dim, int n) {
     const int lane = threadIdx.x & 31, j = lane & 7;
-    const bool whole = g.whole();
     const int rows = min(32, g.s.n * a.H - (g.mt * TT_M + row0));  // that exist
-    // this lane's 16-byte chunk of rows lane / 8, + 4, ..: of 32 fp32, or of 32 hi and 32 lo halves
-    char *dst;
-    size_t pitch, step;
-    if (whole) {
-        dst = reinterpret_cast<char *>(
-            a.olat2 + ((size_t)g.s.first * a.H + g.mt * TT_M + row0) * 2 * TT_DL + dim);
-        dst += (j & 3) * 16 + (j >> 2) * TT_DL * 2;
-        pitch = TT_DL * 4;
-        step = 64;
-    } else {
-        dst = reinterpret_cast<char *>(a.part + ((size_t)g.slot(cl) * TT_M + row0) * TT_PART + dim);
-        dst += j * 16;
-        pitch = TT_PART * 4;
-        step = 128;
-    }
-    dst += (lane >> 3) * pitch;
+    if (!g.whole()) {
+        float4 *dst = reinterpret_cast<float4 *>(a.part + (size_t)g.slot(cl) * TT_PART) +
+                      dim / 4 * TT_M + row0 + lane;
 #pragma unroll 1
-    for (int c = 0; c < n; c += 32, dst += step) {
+        for (int c = 0; c < n; c += 16, dst += 4 * TT_M) {
+            float v[16];
+            tmem_ld16(addr + c, v);
+            tmem_wait_ld();
+            if (lane < rows) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    dst[i * TT_M] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            }
+        }
+        return;
+    }
+    // this lane's 16-byte chunk of rows lane / 8, + 4, ..: of 32 hi and 32 lo halves
+    char *dst = reinterpret_cast<char *>(
+        a.olat2 + ((size_t)g.s.first * a.H + g.mt * TT_M + row0) * 2 * TT_DL + dim);
+    dst += (j & 3) * 16 + (j >> 2) * TT_DL * 2 + (lane >> 3) * TT_DL * 4;
+#pragma unroll 1
+    for (int c = 0; c < n; c += 32, dst += 64) {
         float v[32];
         tmem_ld32(addr + c, v);
         tmem_wait_ld();
-        if (whole) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint4 hi = pack_bf8(v + 8 * i);
-                float h[8], lo[8];
-                unpack_bf8(hi, h);
+        for (int i = 0; i < 4; i++) {
+            const uint4 hi = pack_bf8(v + 8 * i);
+            float h[8], lo[8];
+            unpack_bf8(hi, h);
 #pragma unroll
-                for (int k = 0; k < 8; k++) lo[k] = v[8 * i + k] - h[k];
-                st16s(stage + swz(lane, i), hi);
-                st16s(stage + swz(lane, 4 + i), pack_bf8(lo));
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                st16s(stage + swz(lane, i),
-                      make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]),
-                                 __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3])));
+            for (int k = 0; k < 8; k++) lo[k] = v[8 * i + k] - h[k];
+            st16s(stage + swz(lane, i), hi);
+            st16s(stage + swz(lane, 4 + i), pack_bf8(lo));
         }
         __syncwarp();
         char *d = dst;
 #pragma unroll
-        for (int i = 0; i < 8; i++, d += 4 * pitch) {
+        for (int i = 0; i < 8; i++, d += 4 * TT_DL * 4) {
             const int r = 4 * i + (lane >> 3);
             if (r < rows)
                 *reinterpret_cast<uint4 *>(d) = *reinterpret_cast<const uint4 *>(stage + swz(r, j));
@@ -628,9 +631,9 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
             const float lt = l + o;
             if (sg.whole()) a.rowsum[(size_t)sg.s.first * a.H + lr] = lt;
             else {
-                float *dst = a.part + ((size_t)sg.slot(cl) * TT_M + row) * TT_PART + TT_DL;
-                dst[0] = m_ref;
-                dst[1] = lt;
+                float *dst = a.part + (size_t)sg.slot(cl) * TT_PART + row;
+                dst[TT_PART_M] = m_ref;
+                dst[TT_PART_L] = lt;
             }
         }
     }
@@ -712,6 +715,8 @@ __device__ __forceinline__ void value_mma(const TreeArgs &a, TreeWalk walk, uint
 // Bring the rows of the tiles to come into L2 (both CTAs' loads find them there): the score CTA's
 // stages do not cover the latency of HBM under load, about 3000 cycles. Plain prefetches: TMA's take
 // as much of its time as the loads. The score CTA's loads run two to three tiles before this CTA's.
+// At the start the clusters' first tiles share HBM's rate, so the others wait: TT_PACE is what it takes
+// to bring one tile to every cluster (without the wait the first scores came 15000 cycles later).
 __device__ __forceinline__ void value_prefetch(const TreeArgs &a, TreeWalk walk, TreeBars &bars) {
     const int lane = threadIdx.x & 31, box = min(a.v.page_size, TT_TILE);
     const long long t0 = clock64();
@@ -723,6 +728,7 @@ __device__ __forceinline__ void value_prefetch(const TreeArgs &a, TreeWalk walk,
                 __nanosleep(400);
                 if (*(volatile unsigned *)a.err || clock64() - t0 > wait_limit(a.err)) return;
             }
+            if (g > 0 && g <= TT_AHEAD) __nanosleep(TT_PACE);
             const int end = min((t + 1) * TT_TILE, sg.s.len + sg.s.n);
             for (int p = t * TT_TILE; p < end; p += box) {
                 const long long row = paged_row(a.v, sg.b, p);
@@ -873,68 +879,69 @@ mla_tree_attend_tc(const __grid_constant__ TreeMaps maps, const __grid_constant_
     if (warp == 1) tmem_dealloc(tbase, TT_TM_COLS);
 }
 
-// Join the row tiles that several clusters took (the flash-decoding identity), a row per warp and
-// round: the lanes take the parts' (m, l) first, then float4s lane, lane + 32, .. of every part.
-// Bound by L2's latency: with a row per block of 128 threads it took 16 us for 73 cut tiles, and two
-// rounds of rows take the place of eight now.
-constexpr int TJ_WARPS = 4;
+// Join the row tiles that several clusters took (the flash-decoding identity). A warp takes 8 dims of
+// 32 rows, a row to a lane, as the partials lie, TJ_UP parts at a time with a running maximum. Bound by
+// L2's latency: a warp has few items after one another and few loads that wait for others (a row per
+// block of 128 threads took 16 us for 73 cut tiles).
+constexpr int TJ_WARPS = 4, TJ_UP = 4;
+constexpr int TJ_ITEMS = TT_M / 32 * (TT_DL / 8);  // of a cut row tile
 __global__ void __launch_bounds__(TJ_WARPS * 32, 8) mla_tree_join(const __grid_constant__ TreeArgs a) {
     pdl_trigger();
     pdl_wait();
-    const int lane = threadIdx.x & 31, items = a.plan->cuts * TT_M;
-    const size_t stride = (size_t)2 * TT_M * TT_PART;  // between clusters
+    const int lane = threadIdx.x & 31, items = a.plan->cuts * TJ_ITEMS;
     for (int i = blockIdx.x * TJ_WARPS + (threadIdx.x >> 5); i < items; i += gridDim.x * TJ_WARPS) {
-        const TreeCut cut = a.plan->cut[i / TT_M];
-        const int row = i % TT_M, c = cut.first;
+        const TreeCut cut = a.plan->cut[i / TJ_ITEMS];
+        const int row = i % (TT_M / 32) * 32 + lane, dim = i % TJ_ITEMS / (TT_M / 32) * 8;
         if (row >= cut.rows) continue;
-        const float *base = a.part + (size_t)row * TT_PART;
-        auto part = [&](int k) { return base + k * stride + (k == c ? TT_M * TT_PART : 0); };
-        float M = -INFINITY;
-        for (int k = c + lane; k <= cut.last; k += 32) M = fmaxf(M, part(k)[TT_DL]);
+        float M = -INFINITY, L = 0.f, o[8] = {};
+        for (int k0 = cut.first; k0 <= cut.last; k0 += TJ_UP) {
+            float m[TJ_UP], l[TJ_UP];
+            float4 v[TJ_UP][2];
 #pragma unroll
-        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        float L = 0.f, o[4][4] = {};
-        for (int k0 = c; k0 <= cut.last; k0 += 32) {
-            float w = 0.f, pl = 0.f;
-            if (k0 + lane <= cut.last) {
-                const float *p = part(k0 + lane);
-                const float m = p[TT_DL];
-                pl = p[TT_DL + 1];
-                w = m == -INFINITY && pl == 0.f ? 0.f : exp2f(m - M);
+            for (int u = 0; u < TJ_UP; u++) {
+                const int k = k0 + u;
+                m[u] = -INFINITY;
+                l[u] = 0.f;
+                v[u][0] = v[u][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (k > cut.last) continue;
+                // the first cluster's part is its odd slot, the others' the even ones
+                const float *p = a.part + (size_t)(2 * k + (k == cut.first)) * TT_PART;
+                m[u] = p[TT_PART_M + row];
+                l[u] = p[TT_PART_L + row];
+                v[u][0] = reinterpret_cast<const float4 *>(p)[dim / 4 * TT_M + row];
+                v[u][1] = reinterpret_cast<const float4 *>(p)[(dim / 4 + 1) * TT_M + row];
             }
-            pl *= w;
+            float M1 = M;
 #pragma unroll
-            for (int s = 16; s; s >>= 1) pl += __shfl_xor_sync(0xffffffffu, pl, s);
-            L += pl;
-            const int n = min(32, cut.last + 1 - k0);
-#pragma unroll 2
-            for (int k = 0; k < n; k++) {
-                const float4 *p = reinterpret_cast<const float4 *>(part(k0 + k)) + lane;
-                const float wk = __shfl_sync(0xffffffffu, w, k);
+            for (int u = 0; u < TJ_UP; u++) M1 = fmaxf(M1, m[u]);
+            const float f = M == M1 ? 1.f : exp2f(M - M1);
+            M = M1;
+            L *= f;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float4 v = p[32 * j];
-                    o[j][0] = fmaf(wk, v.x, o[j][0]);
-                    o[j][1] = fmaf(wk, v.y, o[j][1]);
-                    o[j][2] = fmaf(wk, v.z, o[j][2]);
-                    o[j][3] = fmaf(wk, v.w, o[j][3]);
+            for (int e = 0; e < 8; e++) o[e] *= f;
+#pragma unroll
+            for (int u = 0; u < TJ_UP; u++) {
+                const float w = m[u] == -INFINITY && l[u] == 0.f ? 0.f : exp2f(m[u] - M);
+                L += w * l[u];
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    o[4 * j] = fmaf(w, v[u][j].x, o[4 * j]);
+                    o[4 * j + 1] = fmaf(w, v[u][j].y, o[4 * j + 1]);
+                    o[4 * j + 2] = fmaf(w, v[u][j].z, o[4 * j + 2]);
+                    o[4 * j + 3] = fmaf(w, v[u][j].w, o[4 * j + 3]);
                 }
             }
         }
         const size_t th = (size_t)cut.row0 + row;
-        __nv_bfloat16 *dst = a.olat2 + th * 2 * TT_DL;
+        uint4 *dst = reinterpret_cast<uint4 *>(a.olat2 + th * 2 * TT_DL + dim);
+        const uint4 hi = pack_bf8(o);
+        float h[8], lo[8];
+        unpack_bf8(hi, h);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            float lo[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                lo[e] = o[j][e] - __bfloat162float(__float2bfloat16_rn(o[j][e]));
-            reinterpret_cast<uint2 *>(dst)[lane + 32 * j] =
-                make_uint2(pack_bf2(o[j][0], o[j][1]), pack_bf2(o[j][2], o[j][3]));
-            reinterpret_cast<uint2 *>(dst + TT_DL)[lane + 32 * j] =
-                make_uint2(pack_bf2(lo[0], lo[1]), pack_bf2(lo[2], lo[3]));
-        }
-        if (lane == 0) a.rowsum[th] = L;
+        for (int e = 0; e < 8; e++) lo[e] = o[e] - h[e];
+        dst[0] = hi;
+        dst[TT_DL / 8] = pack_bf8(lo);
+        if (dim == 0) a.rowsum[th] = L;
     }
 }
 
@@ -964,7 +971,7 @@ static TreeWs tree_ws(int B, int T, int H) {
     w.cum = take(((size_t)B + 1) * sizeof(long long));
     w.keep = take((size_t)T * sizeof(int));
     w.qlat = take((size_t)T * H * TT_QW * 2);
-    w.part = take((size_t)2 * TT_CLUSTERS * TT_M * TT_PART * sizeof(float));
+    w.part = take((size_t)2 * TT_CLUSTERS * TT_PART * sizeof(float));
     w.olat2 = take((size_t)T * H * 2 * TT_DL * 2);
     w.rowsum = take((size_t)T * H * sizeof(float));
     w.total = off;
