@@ -106,12 +106,17 @@ struct HeadGemmMaps {
     CUtensorMap a, b;
 };
 
+struct AbsorbMaps {
+    CUtensorMap a, b, rope, out;
+};
+
 // CTA (h, y, z) computes columns [256 z, +256) of q_lat for 128 sequences: a head's 128 KB
 // W_UK block is split over two CTAs, and two CTAs (97 KB of shared memory each) share an SM.
+// The rows leave by TMA from shared memory, 128 bytes of a row at a time: stored by the lanes, 16
+// bytes of 32 rows in each instruction, they took longer than all else (64 tokens of 128 heads: 12 us,
+// now 10; 200 and more: 27 us, now 17).
 __global__ void __launch_bounds__(128, 2)
-mla_q_absorb_tc(const __grid_constant__ HeadGemmMaps maps, const __nv_bfloat16 *__restrict__ q_rope,
-                __nv_bfloat16 *__restrict__ qlat, int pitch, int B, int H,
-                unsigned *__restrict__ err) {
+mla_q_absorb_tc(const __grid_constant__ AbsorbMaps maps, unsigned *__restrict__ err) {
     extern __shared__ uint8_t smraw[];
     uint8_t *sm = (uint8_t *)(((uintptr_t)smraw + 1023) & ~(uintptr_t)1023);
     uint8_t *sA = sm;              // 2 K-blocks x [128 b][128 B]
@@ -157,31 +162,29 @@ mla_q_absorb_tc(const __grid_constant__ HeadGemmMaps maps, const __nv_bfloat16 *
     __syncwarp();
     const bool ok = warp_wait(&bar_mma, 0, err, 0x402);
     tc_fence_after();
-    const int b = b0 + 32 * warp + (tid & 31);
-    if (ok) {
-        for (int c = 0; c < 256; c += 16) {
-            float v[16];
-            tmem_ld16(tb + ((uint32_t)(32 * warp) << 16) + c, v);
+    if (ok) {  // the same for every warp, but for a wait that ran out
+        if (tid == 0 && z == 0) {  // q_rope's block through the queries' place
+            mbar_expect_tx(&bar_ld, 16384);
+            tma_load_3d(sA, &maps.rope, &bar_ld, 0, h, b0);
+        }
+        const int row = tid;  // 32 warp + lane: TMEM's
+        for (int c = 0; c < 256; c += 32) {
+            float v[32];
+            tmem_ld32(tb + ((uint32_t)(32 * warp) << 16) + c, v);
             tmem_wait_ld();
-            if (b < B) {
-                uint32_t pk[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const __nv_bfloat162 t2 = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-                    pk[i] = *reinterpret_cast<const uint32_t *>(&t2);
-                }
-                uint4 *dst = reinterpret_cast<uint4 *>(qlat + ((size_t)b * pitch + h) * MLA_QW + 256 * z +
-                                                       c);
-                dst[0] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-                dst[1] = make_uint4(pk[4], pk[5], pk[6], pk[7]);
-            }
+            for (int i = 0; i < 4; i++)
+                st16s(sB + (c / 64) * 16384 + swz(row, (c % 64) / 8 + i), pack_bf8(v + 8 * i));
         }
-        if (b < B && z == 0) {
-            const uint4 *src = reinterpret_cast<const uint4 *>(q_rope + ((size_t)b * H + h) * MLA_DR);
-            uint4 *dst = reinterpret_cast<uint4 *>(qlat + ((size_t)b * pitch + h) * MLA_QW + MLA_DL);
-#pragma unroll
-            for (int i = 0; i < MLA_DR / 8; i++) dst[i] = src[i];
-        }
+        fence_async_shared();
+    }
+    __syncthreads();
+    if (tid == 0 && ok) {
+        for (int nb = 0; nb < 4; nb++)
+            tma_store_3d(&maps.out, sB + nb * 16384, 256 * z + 64 * nb, h, b0);
+        if (z == 0 && mbar_wait(&bar_ld, 1, err, 0x403)) tma_store_3d(&maps.out, sA, MLA_DL, h, b0);
+        bulk_commit();
+        bulk_wait();
     }
     tc_fence_before();
     __syncthreads();
@@ -1055,18 +1058,24 @@ int mla_absorb(k3cuda_ctx *ctx, __nv_bfloat16 *qlat, int pitch, const void *q_no
         return launch_pdl(ctx, ctx->stream, nm, mla_q_absorb_small<8>, g, blk, 0, qn, qr, wk, uk,
                           qlat, pitch, B, H);
     }
-    HeadGemmMaps maps;
+    AbsorbMaps maps;
     int rc = make_tmap_3d(&maps.a, q_nope, BF, 2, MLA_DN, H, B, MLA_DN * 2,
                           (uint64_t)H * MLA_DN * 2, 64, 1, 128);
     if (!rc)
         rc = make_tmap_3d(&maps.b, w_uk, BF, 2, MLA_DL, MLA_DN, H, MLA_DL * 2,
                           (uint64_t)uk_head_rows * MLA_DL * 2, 64, 64, 1);
+    if (!rc)
+        rc = make_tmap_3d(&maps.rope, q_rope, BF, 2, MLA_DR, H, B, MLA_DR * 2,
+                          (uint64_t)H * MLA_DR * 2, 64, 1, 128);
+    if (!rc)
+        rc = make_tmap_3d(&maps.out, qlat, BF, 2, MLA_QW, H, B, MLA_QW * 2,
+                          (uint64_t)pitch * MLA_QW * 2, 64, 1, 128);
     if (rc) return rc;
     const int smem = 2 * 16384 + 8 * 8192 + 1024;
     if ((rc = set_smem(mla_q_absorb_tc, smem))) return rc;
     const dim3 grid(H, (B + 127) / 128, 2);  // two 256-column halves of q_lat per head
     return launch_pdl(ctx, ctx->stream, "mla_q_absorb_tc", mla_q_absorb_tc, grid, dim3(128), smem,
-                      maps, qr, qlat, pitch, B, H, ctx->err_word);
+                      maps, ctx->err_word);
 }
 
 // out[b][h] = W_UV[h] o_lat[b][h] / rowsum[b][h], o_lat as bf16 hi/lo pairs [B][H][2 MLA_DL];
@@ -1095,8 +1104,8 @@ int mla_project(k3cuda_ctx *ctx, void *out, int out_dtype, const __nv_bfloat16 *
                           (uint64_t)uv_head_rows * MLA_DL * 2, 64, 128, 1);
     if (rc) return rc;
     const dim3 grid(H, (B + 127) / 128);
-    const int smem = 3 * 2 * 16384 + 1024;
     const char *nm = "mla_project_tc";
+    const int smem = 3 * 2 * 16384 + 1024;
     if (bf) {
         if ((rc = set_smem(mla_project_tc<__nv_bfloat16>, smem))) return rc;
         return launch_pdl(ctx, ctx->stream, nm, mla_project_tc<__nv_bfloat16>, grid, dim3(128), smem,
