@@ -257,8 +257,8 @@ typedef struct {
 /* The new tokens of B sequences, packed: sequence b has cu_tokens[b+1] - cu_tokens[b] of them
  * (none is allowed), rows cu_tokens[b].. of the T rows of every per-token array, and cache
  * positions ctx_lens[b].. behind its ctx_lens[b] cached rows (0 is allowed). ctx_lens d [B],
- * cu_tokens d [B + 1], rising, cu_tokens[B] <= T. Rows from cu_tokens[B] on are padding: they are
- * neither read nor written.
+ * cu_tokens d [B + 1], rising, cu_tokens[B] <= T. Rows from cu_tokens[B] on are padding: what they
+ * hold does not matter, and outputs' rows there stay as they were.
  *
  * page_table, ctx_lens and cu_tokens are DEVICE arrays, read when the kernels run: a captured
  * graph replays with what they hold then. The kernels check them. A sequence that breaks a rule
@@ -302,8 +302,8 @@ int k3cuda_mla_paged_append(k3cuda_ctx *ctx, const k3cuda_paged_cache *cache,
  * At most K3CUDA_MAX_DRAFTS new tokens per sequence. A token that sees nothing (no cached row,
  * no bit) gives zeros. What hidden or unwritten cache rows hold does not matter, infinities and
  * NaN included; a visible draft row that holds one gives NaN. Supported: dn == dv == 128,
- * dr == 64, dl == 512, H <= 128. workspace d: k3cuda_mla_tree_attend_workspace() bytes, 256-byte
- * aligned, used by one call at a time. */
+ * dr == 64, dl == 512, H <= 128, scale finite. workspace d: k3cuda_mla_tree_attend_workspace()
+ * bytes, 256-byte aligned, used by one call at a time. */
 #define K3CUDA_MAX_DRAFTS 64
 int k3cuda_mla_tree_attend_workspace(int B, int T, int H, int dl, int dv, size_t *bytes);
 int k3cuda_mla_tree_attend(k3cuda_ctx *ctx, void *out, int out_dtype, const void *q_nope,

@@ -1003,6 +1003,8 @@ extern "C" int k3cuda_mla_tree_attend(k3cuda_ctx *ctx, void *out, int out_dtype,
     if (rc || (rc = tree_shape(batch->B, batch->T, H, dn, dr, dl, dv))) return rc;
     K3_ARG_CHECK(out_dtype == K3CUDA_F32 || out_dtype == K3CUDA_BF16, "%s: bad out_dtype %d", what,
                  out_dtype);
+    const float scale_log2e = scale * 1.4426950408889634f;
+    K3_ARG_CHECK(isfinite(scale_log2e), "%s: bad scale %g", what, scale);
     const int B = batch->B, T = batch->T;
     if (B == 0 || T == 0) return enter(ctx);
     K3_ARG_CHECK(out && q_nope && q_rope && w_uk && w_uv, "%s: null pointer", what);
@@ -1025,7 +1027,7 @@ extern "C" int k3cuda_mla_tree_attend(k3cuda_ctx *ctx, void *out, int out_dtype,
     const TreeArgs a{paged_view(cache, batch), plan, tree_mask,
                      (const __nv_bfloat16 *)cache->latent, (const __nv_bfloat16 *)cache->rope, qlat,
                      (float *)(w + ws.part), (__nv_bfloat16 *)(w + ws.olat2),
-                     (float *)(w + ws.rowsum), H, scale * 1.4426950408889634f, ctx->err_word};
+                     (float *)(w + ws.rowsum), H, scale_log2e, ctx->err_word};
     const uint64_t rows = (uint64_t)cache->n_pages * cache->page_size;
     const uint32_t kbox = cache->page_size < TT_TILE ? cache->page_size : TT_TILE;
     const uint32_t vbox = cache->page_size < TT_VROWS ? cache->page_size : TT_VROWS;

@@ -123,6 +123,14 @@ def test_attend_refusals(kw, code, text):
 
 
 @pytest.mark.parametrize("kw,code,text", [
+    (dict(ws=None), k3cuda.ERR_WORKSPACE, "workspace"), (dict(nws=1000), k3cuda.ERR_WORKSPACE, "workspace"),
+    (dict(ws=P + 64), k3cuda.ERR_ARG, "256-byte"), (dict(scale=float("nan")), k3cuda.ERR_ARG, "scale"),
+    (dict(scale=float("-inf")), k3cuda.ERR_ARG, "scale"), (dict(scale=3e38), k3cuda.ERR_ARG, "scale")])
+def test_attend_refuses_its_workspace_and_scale(kw, code, text):
+    refused(attend(cache(), batch(), **kw), code, text)
+
+
+@pytest.mark.parametrize("kw,code,text", [
     (dict(T=-1), k3cuda.ERR_ARG, "T=-1"), (dict(V=0), k3cuda.ERR_ARG, "V=0"),
     (dict(V=(1 << 24) + 1, stride=1 << 25), k3cuda.ERR_UNSUPPORTED, "not built"),
     (dict(K=33), k3cuda.ERR_ARG, "K=33"), (dict(K=-1), k3cuda.ERR_ARG, "K=-1"),

@@ -314,6 +314,18 @@ def test_tree_pages(ctx, page):
                k3cuda.BF16)
 
 
+@pytest.mark.parametrize("len0", [74 * 128 - 1, 74 * 128])
+def test_tree_a_tile_for_each_cluster_and_one_more(ctx, len0):
+    rng = np.random.default_rng(len0)
+    check_tree(ctx, rng, [len0], [1], 128, 16, "tree")
+
+
+def test_tree_drafts_across_tiles(ctx):
+    """Drafts that end one tile and begin the next, 32-row chunks without a row, with one, full."""
+    rng = np.random.default_rng(21)
+    check_tree(ctx, rng, [100, 127, 96, 31, 32, 33, 65], [60, 64, 33, 1, 32, 2, 63], 8, 6, "tree")
+
+
 def test_tree_sees_nothing(ctx):
     rng = np.random.default_rng(8)
     *_, got = check_tree(ctx, rng, [0, 0, 5], [3, 1, 2], 16, 5, "none")
@@ -575,6 +587,20 @@ def test_logprobs_odd_rows(ctx, bf16, V):
     assert lp[8, 4] == 0 and ent[8] == 0
     again = run_lp(ctx, x, tokens, 30, bf16, entropy=False)
     assert (again[2] == ids).all() and np.array_equal(again[0], lp, equal_nan=True)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("T,V", [(1, 163840), (620, 20000), (100, 30001)])
+def test_logprobs_few_tokens_allowed(ctx, bf16, T, V):
+    """All but a few tokens forbidden: warps, blocks and segments without one, or with one thread's."""
+    rng = np.random.default_rng([T, V])
+    x = np.full((T, V), -np.inf, np.float32)
+    for r in range(T):
+        n = [1, 5, 300, 4000][r % 4 if T > 1 else 2]
+        at = rng.integers(0, V, n) if r % 8 < 4 else (17 + 256 * np.arange(n)) % V
+        x[r, at] = rng.standard_normal(n) * 3
+    x = W.round_bf16(x) if bf16 else x
+    check_lp(ctx, x, rng.integers(0, V, (T, 2)), 32 if T == 1 else 8, bf16)
 
 
 def test_logprobs_nothing_to_do(ctx):
