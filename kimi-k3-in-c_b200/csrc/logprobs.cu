@@ -460,7 +460,7 @@ static LpPlan lp_plan(int T, int V, int io_dtype) {
     LpPlan p;
     p.U = T * ((nv + 4 * LP_THREADS - 1) / (4 * LP_THREADS)) >= want ? 4 : 1;
     const long long its = (nv + p.U * LP_THREADS - 1) / (p.U * LP_THREADS);
-    long long S = (want + T - 1) / (T > 0 ? T : 1);
+    long long S = T > 0 && T < want ? want / T : 1;
     S = S < its ? S : its;
     S = S < LP_MAX_SEG ? S : LP_MAX_SEG;
     if ((its + S - 1) / S > LP_MAX_IT) S = (its + LP_MAX_IT - 1) / LP_MAX_IT;
