@@ -18,6 +18,12 @@
 //
 // Rows are cut into segments of whole iterations when there are few of them: each block leaves
 // (m, s, t) and its K best, and a second kernel joins a row's segments.
+//
+// Measured: 512 rows of 163840 fp32 logits with the 20 likeliest 69 us (4.9 TB/s, 75 % of a copy's
+// rate; 59 us without the likeliest, whose work leaves a block's loads idle meanwhile); 2048 rows of
+// 163840 bf16 124 us (5.4 TB/s; the exponentials' unit is 68 % busy); one such row 10 us. Blocks that
+// begin their next segment's loads before they finish the last were slower (124 -> 149 us: segments
+// are dealt out unevenly then), and so was one segment instead of two for 512 rows (72 us).
 #include "internal.cuh"
 #include "sm100.cuh"
 

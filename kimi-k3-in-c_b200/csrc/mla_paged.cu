@@ -10,7 +10,9 @@
 //
 // Memory-bound: every value is read once and written once. One block per (token, 16 heads) and
 // one per token for the cache row, 128 threads with all loads of a thread issued before any
-// use; a token's 32 angles are formed once per block.
+// use; a token's 32 angles are formed once per block. Measured: 5058 tokens of 128 heads in fp32
+// 137 us, 5.6 TB/s of what has to be read and written (86 % of a copy's rate); 64 tokens of 16 heads
+// 7 us, of which the host's part of the call is most.
 #include "internal.cuh"
 #include "paged.cuh"
 
