@@ -323,8 +323,8 @@ int k3cuda_mla_tree_attend(k3cuda_ctx *ctx, void *out, int out_dtype, const void
  * in one pass over the logits, sums in fp32. A logit of -inf is a token that cannot come. A row
  * that holds a NaN or +inf, or nothing but -inf, has no distribution: NaN, ids -1.
  * K <= K3CUDA_MAX_TOP, V >= 1, any alignment of the rows to their element size. workspace d:
- * k3cuda_token_logprobs_workspace() bytes (may be 0), 256-byte aligned, used by one call at a
- * time. */
+ * k3cuda_token_logprobs_workspace() bytes (which do for smaller T, V and K too), 256-byte aligned,
+ * used by one call at a time. */
 #define K3CUDA_MAX_TOP 32
 int k3cuda_token_logprobs_workspace(int T, int V, int K, size_t *bytes);
 int k3cuda_token_logprobs(k3cuda_ctx *ctx, const void *logits, int io_dtype, long long row_stride,

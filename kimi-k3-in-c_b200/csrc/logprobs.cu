@@ -24,6 +24,8 @@
 // 163840 bf16 124 us (5.4 TB/s; the exponentials' unit is 68 % busy); one such row 10 us. Blocks that
 // begin their next segment's loads before they finish the last were slower (124 -> 149 us: segments
 // are dealt out unevenly then), and so was one segment instead of two for 512 rows (72 us).
+#include <algorithm>
+
 #include "internal.cuh"
 #include "sm100.cuh"
 
@@ -459,10 +461,11 @@ struct LpPlan {
 
 // Blocks to fill the GPU once (four an SM) where the rows allow it, on a B200's 148 SMs
 // whatever the device, so that the workspace query needs no device.
+constexpr int LP_BLOCKS = 148 * 4;
 static LpPlan lp_plan(int T, int V, int io_dtype) {
     const int N = io_dtype == K3CUDA_F32 ? 4 : 8;
     const long long nv = ((long long)V + 2 * N - 2) / N;  // most vectors, whatever the skew
-    constexpr long long want = 148 * 4;
+    constexpr long long want = LP_BLOCKS;
     LpPlan p;
     p.U = T * ((nv + 4 * LP_THREADS - 1) / (4 * LP_THREADS)) >= want ? 4 : 1;
     const long long its = (nv + p.U * LP_THREADS - 1) / (p.U * LP_THREADS);
@@ -486,9 +489,21 @@ static int lp_shape(int T, int V, int K) {
     return K3CUDA_OK;
 }
 
-static size_t lp_bytes(const LpPlan &p, int T, int K) {
-    if (p.S == 1 || T == 0) return 0;
-    return lp_align((size_t)T * p.S * sizeof(Stat)) + lp_align((size_t)T * p.S * K * sizeof(u64));
+static size_t lp_bytes(long long segments, int K) {
+    return lp_align(segments * sizeof(Stat)) + lp_align(segments * K * sizeof(u64));
+}
+static size_t lp_need(const LpPlan &p, int T, int K) {
+    return p.S == 1 || T == 0 ? 0 : lp_bytes((long long)T * p.S, K);
+}
+// What no call of up to T rows of up to V logits passes: LP_BLOCKS segments, or those that LP_MAX_IT
+// cuts every row into.
+static size_t lp_bound(int T, int V, int K, int io_dtype) {
+    if (T == 0) return 0;
+    const int N = io_dtype == K3CUDA_F32 ? 4 : 8;
+    const long long nv = ((long long)V + 2 * N - 2) / N;
+    const long long its = (nv + 4 * LP_THREADS - 1) / (4 * LP_THREADS);
+    const long long cut = (its + LP_MAX_IT - 1) / LP_MAX_IT;
+    return lp_bytes(std::max<long long>(LP_BLOCKS, cut > 1 ? T * cut : 0), K);
 }
 
 template <typename T> static int lp_run(k3cuda_ctx *ctx, const LpArgs &a, const LpPlan &p) {
@@ -511,9 +526,7 @@ extern "C" int k3cuda_token_logprobs_workspace(int T, int V, int K, size_t *byte
     K3_ARG_CHECK(bytes, "token_logprobs: null bytes");
     int rc = lp_shape(T, V, K);
     if (rc) return rc;
-    const size_t a = lp_bytes(lp_plan(T, V, K3CUDA_F32), T, K);
-    const size_t b = lp_bytes(lp_plan(T, V, K3CUDA_BF16), T, K);
-    *bytes = a > b ? a : b;
+    *bytes = std::max(lp_bound(T, V, K, K3CUDA_F32), lp_bound(T, V, K, K3CUDA_BF16));
     return K3CUDA_OK;
 }
 
@@ -531,7 +544,7 @@ extern "C" int k3cuda_token_logprobs(k3cuda_ctx *ctx, const void *logits, int io
                  "token_logprobs: bad G=%d or null output", G);
     K3_ARG_CHECK(row_stride >= V, "token_logprobs: row_stride=%lld < V=%d", row_stride, V);
     const LpPlan p = lp_plan(T, V, io_dtype);
-    const size_t need = lp_bytes(p, T, K);
+    const size_t need = lp_need(p, T, K);
     if (need && (!workspace || workspace_bytes < need))
         return set_error(K3CUDA_ERR_WORKSPACE, "token_logprobs: workspace %zu < %zu",
                          workspace_bytes, need);

@@ -175,6 +175,19 @@ def test_workspace_queries():
         last = n.value
 
 
+def test_logprobs_workspace_holds_for_smaller_calls():
+    n = C.c_size_t()
+    for V in (1, 777, 50257, 163841, 1 << 24):
+        for T in (1, 2, 300, 591, 592, 700, 5000):
+            k3cuda.check(k3cuda.lib().k3cuda_token_logprobs_workspace(T, V, 20, C.byref(n)))
+            for T1 in {1, 2, 3, T // 7 + 1, T // 2 + 1, T}:
+                for V1 in {1, V // 9 + 1, V // 2 + 1, V}:
+                    for dt in (k3cuda.F32, k3cuda.BF16):
+                        if T1 <= T:
+                            refused(logprobs(T=T1, V=V1, stride=V1, K=19, dt=dt, nws=n.value),
+                                    k3cuda.ERR_ARG, "null context")
+
+
 SRC = r"""
 #include <assert.h>
 #include <stdio.h>
