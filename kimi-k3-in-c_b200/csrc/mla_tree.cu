@@ -31,8 +31,9 @@
 //     so a chunk comes in one, through a four-dimensional view of the cache that lays eight-row
 //     groups [dim blocks][8 rows][128 B] one after another; pages of fewer rows take one each.
 // Per SM:
-//   score   TMEM: query 256 columns, S 2 x 128;  shared: a tile in 4 stages of 32 KB (128 rows x 128
-//           dims, K-major), its rope dims 16 KB, the query's 16 KB, P 32 KB on its way out
+//   score   TMEM: query 256 columns, S 2 x 128;  shared: 5 stages of 32 KB (128 rows x 128 dims,
+//           K-major, a quarter of a tile), the tile's rope dims 16 KB, the query's 16 KB, P 32 KB on its
+//           way out (four stages and no reading ahead in the page table: 64 x 1 193 us, now 188)
 //   value   TMEM: o 512 columns;  shared: a tile in 4 stages of 32 KB (32 rows x 512 dims, MN-major),
 //           P 2 x 32 KB
 // Warps: 0 loads (a lane per page), 1 issues the MMAs, 2-9 are two groups of one warp per lane
@@ -48,12 +49,14 @@
 // The line is formed on the device from the batch's tables (mla_tree_plan), so that a captured
 // call follows them.
 //
-// Measured (the five launches of a call): 64 x 1 token of 128 heads over 8192 rows 192 us, of which this
-// kernel 162 (its floor is 97 us of HBM and 91 of MMAs); 48 x 13 tokens, 128 heads, 350 to 400 us as the
+// Measured (the five launches of a call): 64 x 1 token of 128 heads over 8192 rows 188 us, of which this
+// kernel 160 (its floor is 97 us of HBM and 91 of MMAs); 48 x 13 tokens, 128 heads, 350 to 400 us as the
 // clock allows (300 in this kernel; 181 us of MMAs); one token after 509 rows 26 us. A tile takes about
-// 4300 cycles where its MMAs in the score CTA need 2650: without the loads of the rows it would be 3550,
-// without the softmax 3150. Both share shared memory's 128 B a clock with the MMAs' reads of the rows
-// (360 KB a tile in all, 2800 cycles at best). A row tile's start and end take some 14000 cycles.
+// 4250 cycles where its MMAs in the score CTA need 2650. What it waits for are the rows: 163 KB at 55 B a
+// clock, which share shared memory's 128 with the MMAs' reads of them and with P, and 91 cycles for each
+// of 10 TMA instructions (two pages of 64 rows; 18 instructions, a block of 64 dims each: 4600). 3870 of
+// the 4250 are the SM's own: so much it takes with 12 clusters at work instead of 74. A row tile's
+// start and end take some 14000 cycles.
 //
 // Hidden rows: a masked score gives weight 0 whatever it is, and a zero weight times a row of
 // infinities must stay 0, so in tiles that reach past the cached rows the value CTA zeroes
@@ -72,25 +75,26 @@ constexpr int TT_DN = 128, TT_DR = 64, TT_DL = 512, TT_DV = 128, TT_H = 128;
 constexpr int TT_QW = TT_DL + TT_DR;       // absorbed query width
 constexpr int TT_M = 128;                  // rows of a row tile
 constexpr int TT_TILE = 128;               // cache rows of a tile
-constexpr int TT_KCH = 4, TT_VCH = 4;      // chunks of a tile, one to a stage: by dims, by rows
+constexpr int TT_KCH = 4, TT_VCH = 4;      // chunks of a tile: by dims, by rows
+constexpr int TT_KST = 5, TT_VST = TT_VCH; // stages, a chunk each
 constexpr int TT_KSTAGE = TT_TILE * TT_DL * 2 / TT_KCH;
 constexpr int TT_VROWS = TT_TILE / TT_VCH;
 constexpr int TT_VSTAGE = TT_VROWS * TT_DL * 2;
-constexpr int TT_AHEAD = 4;                // tiles that rows are brought into L2 before their load
+constexpr int TT_AHEAD = 3;                // tiles that rows are brought into L2 before their load
 constexpr int TT_PACE = 1600;              // ns between the first of them
 constexpr int TT_PBUF = 2 * TT_M * 128;    // two blocks of 64 columns
-constexpr int TT_OFF_KR = TT_KCH * TT_KSTAGE;     // score: rope dims of the tile
+constexpr int TT_OFF_KR = TT_KST * TT_KSTAGE;     // score: rope dims of the tile
 constexpr int TT_OFF_QR = TT_OFF_KR + TT_TILE * 128;  // and of the query
 constexpr int TT_OFF_PS = TT_OFF_QR + TT_M * 128;     // P on its way out
 constexpr int TT_OFF_FS = TT_OFF_PS + TT_PBUF;        // its rescale factors
 constexpr int TT_GRP = 2;                  // groups of worker warps, one warp per lane quarter each
 constexpr int TT_OFF_VAL = TT_OFF_FS + TT_M * 4;      // values shared by a row's warps
-constexpr int TT_OFF_P = TT_VCH * TT_VSTAGE;      // value: P, two buffers
+constexpr int TT_OFF_P = TT_VST * TT_VSTAGE;      // value: P, two buffers
 constexpr int TT_OFF_F = TT_OFF_P + 2 * TT_PBUF;  // and their factors
 constexpr int TT_OFF_W = TT_OFF_F + 1024;         // o on its way out, 4 KB a warp
 constexpr int TT_SMEM_SCORE = TT_OFF_VAL + 2 * TT_GRP * TT_M * 4;
 constexpr int TT_SMEM_VALUE = TT_OFF_W + 4 * TT_GRP * 4096;
-constexpr int TT_SMEM = (TT_SMEM_SCORE > TT_SMEM_VALUE ? TT_SMEM_SCORE : TT_SMEM_VALUE) + 1024;
+constexpr int TT_OFF_BARS = TT_SMEM_SCORE > TT_SMEM_VALUE ? TT_SMEM_SCORE : TT_SMEM_VALUE;
 static_assert(TT_OFF_W % 1024 == 0 && 2 * TT_M * 4 <= 1024, "the stages are swizzled");
 
 constexpr int TT_TM_Q = 0, TT_TM_S = 256, TT_TM_COLS = 512;
@@ -296,8 +300,9 @@ __global__ void __launch_bounds__(1024) mla_tree_plan(PagedView v, int H, TreePl
     pdl_wait();
 }
 
-struct TreeBars {
-    uint64_t full[TT_KCH], empty[TT_KCH];  // stages
+struct TreeBars {  // at TT_OFF_BARS
+    uint64_t full[TT_KST], empty[TT_KST];  // stages
+    uint64_t r_full, r_empty;              // score: the tile's rope dims
     uint64_t s_full[2], s_empty[2];        // score
     uint64_t pair[4];                      // score: per lane quarter, its two warps
     uint64_t p_out, p_ack;                 // score: P is written; the peer has it
@@ -307,6 +312,9 @@ struct TreeBars {
     uint32_t tmem_base;
     int tile;                              // value: the tile being loaded
 };
+constexpr int TT_SMEM = TT_OFF_BARS + sizeof(TreeBars);
+static_assert(TT_SMEM <= 232448, "all that a block can have, without slack for the alignment");
+static_assert(TT_VST <= TT_KST, "the value CTA's stages have barriers");
 
 // n columns of o from addr: multiply by f
 __device__ __forceinline__ void rescale_o(uint32_t addr, int n, float f) {
@@ -394,71 +402,89 @@ template <bool kScore>
 __device__ __forceinline__ void tree_loads(const TreeMaps &maps, const TreeArgs &a, TreeWalk walk,
                                            uint8_t *sm, TreeBars &bars) {
     constexpr int CH = kScore ? TT_KCH : TT_VCH, ROWS = kScore ? TT_TILE : TT_VROWS;
+    constexpr int ST = kScore ? TT_KST : TT_VST;
     constexpr int STAGE = kScore ? TT_KSTAGE : TT_VSTAGE, RB = STAGE / ROWS;  // bytes of a row
     const int lane = threadIdx.x & 31;
     const int box = min(a.v.page_size, ROWS), per = ROWS / box;  // rows of a box, boxes of a chunk
-    int k = 0, loaded = 0;  // times the stages were filled; which of them, and in which phase
-    // this lane's box of a tile: its first cache row (page 0 where the table names no page)
-    auto lookup = [&](const TreeSeg &sg, int t) -> int {
+    int g = 0, loaded = 0;  // tiles; stages in use, and their phase
+    int st = 0, fill = 0;   // the next stage and how often it was filled
+    int ropes = 0;          // tiles whose rope dims are loaded
+    // This lane's box of a tile: its page, read a tile before it is looked at (the read takes 700 cycles
+    // and more behind the TMA's traffic, and what waits for it holds up the loads), and its first cache
+    // row (of page 0 where the table names no page).
+    auto box_page = [&](const TreeSeg &sg, int t) -> int {
         const int p = t * TT_TILE + lane * box;
         if (lane >= TT_TILE / box || p >= sg.s.len + sg.s.n) return 0;
-        long long r = paged_row(a.v, sg.b, p);
-        if (r < 0) {
-            if (kScore) atomicCAS(a.err + 1, 0u, (unsigned)PAGED_PAGE);
-            r = p & (a.v.page_size - 1);
-        }
-        return (int)r;
+        return a.v.table[(long long)sg.b * a.v.max_pages + (p >> a.v.shift)];
     };
-    auto free = [&](int c) { return k == 0 || warp_spin(&bars.empty[c], (k - 1) & 1, a.err, 0x501); };
-    auto used = [&](int c) { loaded = (loaded & ~(3 << (2 * c))) | ((k & 1 ? 2 : 1) << (2 * c)); };
+    auto box_row = [&](int page, int t) -> int {
+        if (page < 0 || page >= a.v.n_pages) {
+            if (kScore) atomicCAS(a.err + 1, 0u, (unsigned)PAGED_PAGE);
+            page = 0;
+        }
+        return (page << a.v.shift) + ((t * TT_TILE + lane * box) & (a.v.page_size - 1));
+    };
+    auto free = [&] { return fill == 0 || warp_spin(&bars.empty[st], (fill - 1) & 1, a.err, 0x501); };
+    auto next = [&] {
+        loaded = (loaded & ~(3 << (2 * st))) | ((fill & 1 ? 2 : 1) << (2 * st));
+        if (++st == ST) st = 0, fill++;
+    };
+    // the last tile's products with its rope dims are done
+    auto rope_free = [&] { return g == 0 || warp_spin(&bars.r_empty, (g - 1) & 1, a.err, 0x502); };
     TreeSeg sg;
     bool more = walk.next(sg), ok = true;
-    int t = more ? sg.t0 : 0, row = more ? lookup(sg, t) : 0;
-    for (; more && ok; k++) {
-        const int live = (sg.s.len + sg.s.n - t * TT_TILE + box - 1) / box, at = row;
-        if (!kScore && lane == 0) *(volatile int *)&bars.tile = k;
+    int t = more ? sg.t0 : 0, page = more ? box_page(sg, t) : 0;
+    for (; more && ok; g++) {
+        const int live = (sg.s.len + sg.s.n - t * TT_TILE + box - 1) / box, at = box_row(page, t);
+        if (!kScore && lane == 0) *(volatile int *)&bars.tile = g;
         if (kScore && t == sg.t0) {
             const int q0 = sg.s.first * a.H + sg.mt * TT_M;
 #pragma unroll 1
-            for (int c = 0; c < CH && (ok = free(c)); c++) {
+            for (int c = 0; c < CH && (ok = free()); c++) {
+                const bool rope = c == CH - 1;  // as late as may be: its place is in use longest
+                if (rope && !(ok = rope_free())) break;
                 if (lane == 0) {
-                    mbar_expect_tx(&bars.full[c], STAGE + (c == 0 ? TT_M * 128 : 0));
-                    tma_load_3d(sm + c * STAGE, &maps.q, &bars.full[c], 0, q0, 2 * c);
-                    if (c == 0)
-                        tma_load_2d(sm + TT_OFF_QR, &maps.q_rope, &bars.full[c], TT_DL, q0);
+                    mbar_expect_tx(&bars.full[st], STAGE + (rope ? TT_M * 128 : 0));
+                    tma_load_3d(sm + st * STAGE, &maps.q, &bars.full[st], 0, q0, 2 * c);
+                    if (rope) tma_load_2d(sm + TT_OFF_QR, &maps.q_rope, &bars.full[st], TT_DL, q0);
                 }
                 __syncwarp();
-                used(c);
+                next();
             }
             if (!ok) break;
-            k++;
         }
-        // the next tile's rows, looked up under this one's loads
-        if (++t >= sg.t1) {
-            more = walk.next(sg);
-            t = more ? sg.t0 : 0;
-        }
-        if (more) row = lookup(sg, t);
+        const bool last = t + 1 >= sg.t1;
+        if (!last) page = box_page(sg, ++t);
 #pragma unroll 1
-        for (int c = 0; c < CH && (ok = free(c)); c++) {
+        for (int c = 0; c < CH && (ok = free()); c++) {
             // the lanes whose boxes this chunk takes: all of them, or those of its rows
             const int first = kScore ? 0 : c * per, j = lane - first;
             const int n = max(0, min(per, live - first));
-            const bool rope = kScore && c == 0;
-            if (lane == 0) mbar_expect_tx(&bars.full[c], n * box * (RB + (rope ? 128 : 0)));
+            if (lane == 0) mbar_expect_tx(&bars.full[st], n * box * RB);
             __syncwarp();
-            if (j >= 0 && j < n) {
-                tma_load_4d(sm + c * STAGE + j * box * RB, kScore ? &maps.lat_k : &maps.lat_v,
-                            &bars.full[c], 0, 0, kScore ? c * (RB / 128) : 0, at / 8);
-                if (rope)
-                    tma_load_2d(sm + TT_OFF_KR + j * box * 128, &maps.rope, &bars.full[c], 0, at);
+            if (j >= 0 && j < n)
+                tma_load_4d(sm + st * STAGE + j * box * RB, kScore ? &maps.lat_k : &maps.lat_v,
+                            &bars.full[st], 0, 0, kScore ? c * (RB / 128) : 0, at / 8);
+            next();
+            if (kScore && c == 0) {
+                if (!(ok = rope_free())) break;
+                if (lane == 0) mbar_expect_tx(&bars.r_full, n * box * 128);
+                __syncwarp();
+                if (j < n)
+                    tma_load_2d(sm + TT_OFF_KR + j * box * 128, &maps.rope, &bars.r_full, 0, at);
+                ropes++;
             }
-            used(c);
+        }
+        if (last) {
+            more = walk.next(sg);
+            t = more ? sg.t0 : 0;
+            page = more ? box_page(sg, t) : 0;
         }
     }
     // loads still in flight are waited for (bounded) before the CTA may exit
+    if (ropes && lane == 0) mbar_wait_quiet(&bars.r_full, (ropes - 1) & 1);
     if (lane == 0)
-        for (int c = 0; c < CH; c++)
+        for (int c = 0; c < ST; c++)
             if ((loaded >> (2 * c)) & 3) mbar_wait_quiet(&bars.full[c], (loaded >> (2 * c)) & 2 ? 1 : 0);
     __syncwarp();
 }
@@ -467,8 +493,12 @@ __device__ __forceinline__ void tree_loads(const TreeMaps &maps, const TreeArgs 
 __device__ __forceinline__ void score_mma(const TreeArgs &a, TreeWalk walk, uint8_t *sm,
                                           TreeBars &bars, uint32_t tbase) {
     constexpr uint32_t id = idesc_f16(128, TT_TILE, false, false);
-    int g = 0, k = 0;                // tiles; fillings of the stages (tiles and queries)
-    bool data = false, room = true;  // the next chunk and score buffer, as seen in advance
+    int g = 0, st = 0;                              // tiles; the next stage
+    uint32_t ph = 0;                                // and its phase
+    bool data = false, rope = false, room = true;   // next chunk, rope dims, score buffer: as seen before
+    auto next = [&] {
+        if (++st == TT_KST) st = 0, ph ^= 1;
+    };
     TreeSeg sg;
     while (walk.next(sg)) {
         // The queries into TMEM, 16 dims at a time, once the last row tile's scores are formed. (Taken
@@ -476,42 +506,46 @@ __device__ __forceinline__ void score_mma(const TreeArgs &a, TreeWalk walk, uint
         if (g > 0 && !warp_spin(&bars.s_full[(g - 1) & 1], ((g - 1) >> 1) & 1, a.err, 0x511)) return;
 #pragma unroll 1
         for (int c = 0; c < TT_KCH; c++) {
-            if (!data && !warp_spin(&bars.full[c], k & 1, a.err, 0x514)) return;
+            if (!data && !warp_spin(&bars.full[st], ph, a.err, 0x514)) return;
             tc_fence_after();
-            uint64_t q = sdesc_kmajor(smem_u32(sm + c * TT_KSTAGE));
+            uint64_t q = sdesc_kmajor(smem_u32(sm + st * TT_KSTAGE));
             uint32_t d = tbase + TT_TM_Q + 64 * c;
 #pragma unroll 1
             for (int half = 0; half < 2; half++, q += (TT_M * 128) >> 4, d += 32) {
 #pragma unroll
                 for (int ks = 0; ks < 4; ks++) warp_copy(d + ks * 8, q + ks * (32 >> 4));
             }
-            warp_commit(&bars.empty[c]);
+            warp_commit(&bars.empty[st]);
+            next();
             data = false;
         }
-        k++;
-        for (int t = sg.t0; t < sg.t1; t++, g++, k++) {
+        for (int t = sg.t0; t < sg.t1; t++, g++) {
             const int sb = g & 1;
             const uint32_t d = tbase + TT_TM_S + sb * TT_TILE;
             uint32_t q = tbase + TT_TM_Q;
             if (!room && !warp_spin(&bars.s_empty[sb], ((g >> 1) - 1) & 1, a.err, 0x512)) return;
+            if (!rope && !warp_spin(&bars.r_full, g & 1, a.err, 0x515)) return;
+            tc_fence_after();
+            {
+                const uint64_t qr = sdesc_kmajor(smem_u32(sm + TT_OFF_QR));
+                const uint64_t kr = sdesc_kmajor(smem_u32(sm + TT_OFF_KR));
+#pragma unroll
+                for (int ks = 0; ks < 4; ks++)
+                    warp_mma_ss(d, qr + ks * (32 >> 4), kr + ks * (32 >> 4), id, ks ? 1u : 0u);
+                warp_commit(&bars.r_empty);
+            }
 #pragma unroll 1
             for (int c = 0; c < TT_KCH; c++) {
-                if (!data && !warp_spin(&bars.full[c], k & 1, a.err, 0x513)) return;
+                if (!data && !warp_spin(&bars.full[st], ph, a.err, 0x513)) return;
                 tc_fence_after();
-                uint64_t b = sdesc(smem_u32(sm + c * TT_KSTAGE), 16, 2048);
-                if (c == 0) {
-                    const uint64_t qr = sdesc_kmajor(smem_u32(sm + TT_OFF_QR));
-                    const uint64_t kr = sdesc_kmajor(smem_u32(sm + TT_OFF_KR));
-#pragma unroll
-                    for (int ks = 0; ks < 4; ks++)
-                        warp_mma_ss(d, qr + ks * (32 >> 4), kr + ks * (32 >> 4), id, ks ? 1u : 0u);
-                }
+                uint64_t b = sdesc(smem_u32(sm + st * TT_KSTAGE), 16, 2048);
+                const int used = st;
 #pragma unroll
                 for (int ks = 0; ks < 4; ks++) warp_mma_ts(d, q + ks * 8, b + ks * (32 >> 4), id, 1u);
-                if (c + 1 < TT_KCH) {
-                    data = __all_sync(0xffffffffu, mbar_test(&bars.full[c + 1], k & 1));
-                } else {
-                    data = __all_sync(0xffffffffu, mbar_test(&bars.full[0], (k + 1) & 1));
+                next();
+                data = __all_sync(0xffffffffu, mbar_test(&bars.full[st], ph));
+                if (c + 1 == TT_KCH) {
+                    rope = __all_sync(0xffffffffu, mbar_test(&bars.r_full, (g + 1) & 1));
                     room = g < 1 || __all_sync(0xffffffffu, mbar_test(&bars.s_empty[sb ^ 1],
                                                                           (((g + 1) >> 1) - 1) & 1));
                 }
@@ -521,7 +555,7 @@ __device__ __forceinline__ void score_mma(const TreeArgs &a, TreeWalk walk, uint
                 for (int ks = 0; ks < 4; ks++) warp_mma_ts(d, q + ks * 8, b + ks * (32 >> 4), id, 1u);
                 q += 32;
                 if (c + 1 == TT_KCH) warp_commit(&bars.s_full[sb]);
-                warp_commit(&bars.empty[c]);
+                warp_commit(&bars.empty[used]);
             }
         }
     }
@@ -843,15 +877,20 @@ __device__ __forceinline__ void tree_roles(const TreeMaps &maps, const TreeArgs 
 
 __global__ void __launch_bounds__(TT_THREADS, 1) __cluster_dims__(2, 1, 1)
 mla_tree_attend_tc(const __grid_constant__ TreeMaps maps, const __grid_constant__ TreeArgs a) {
-    extern __shared__ uint8_t smraw[];
-    uint8_t *sm = (uint8_t *)(((uintptr_t)smraw + 1023) & ~(uintptr_t)1023);
-    __shared__ TreeBars bars;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    TreeBars &bars = *reinterpret_cast<TreeBars *>(sm + TT_OFF_BARS);
     const int warp = threadIdx.x >> 5;
     const bool score = cluster_rank() == 0;
     const int cl = blockIdx.x >> 1;
+    if (smem_u32(sm) & 1023) {  // nothing else is in shared memory, so this does not happen
+        if (threadIdx.x == 0) atomicCAS(a.err, 0u, 0x500u);
+        return;
+    }
     pdl_trigger();
     if (threadIdx.x == 0) {
-        for (int c = 0; c < TT_KCH; c++) {
+        mbar_init(&bars.r_full, 1);
+        mbar_init(&bars.r_empty, 1);
+        for (int c = 0; c < TT_KST; c++) {
             mbar_init(&bars.full[c], 1);
             mbar_init(&bars.empty[c], 1);
         }
