@@ -361,10 +361,10 @@ __device__ __forceinline__ void write_o(const TreeArgs &a, const TreeSeg &g, int
     char *dst = reinterpret_cast<char *>(
         a.olat2 + ((size_t)g.s.first * a.H + g.mt * TT_M + row0) * 2 * TT_DL + dim);
     dst += (j & 3) * 16 + (j >> 2) * TT_DL * 2 + (lane >> 3) * TT_DL * 4;
+    float v[32];
+    tmem_ld32(addr, v);
 #pragma unroll 1
     for (int c = 0; c < n; c += 32, dst += 64) {
-        float v[32];
-        tmem_ld32(addr + c, v);
         tmem_wait_ld();
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -377,14 +377,16 @@ __device__ __forceinline__ void write_o(const TreeArgs &a, const TreeSeg &g, int
             st16s(stage + swz(lane, 4 + i), pack_bf8(lo));
         }
         __syncwarp();
+        if (c + 32 < n) tmem_ld32(addr + c + 32, v);  // under the copy
+        uint4 w[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            w[i] = *reinterpret_cast<const uint4 *>(stage + swz(4 * i + (lane >> 3), j));
+        __syncwarp();
         char *d = dst;
 #pragma unroll
-        for (int i = 0; i < 8; i++, d += 4 * TT_DL * 4) {
-            const int r = 4 * i + (lane >> 3);
-            if (r < rows)
-                *reinterpret_cast<uint4 *>(d) = *reinterpret_cast<const uint4 *>(stage + swz(r, j));
-        }
-        __syncwarp();
+        for (int i = 0; i < 8; i++, d += 4 * TT_DL * 4)
+            if (4 * i + (lane >> 3) < rows) *reinterpret_cast<uint4 *>(d) = w[i];
     }
 }
 
