@@ -334,7 +334,8 @@ __device__ __forceinline__ void rescale_o(uint32_t addr, int n, float f) {
 // row0. A lane reads its row from TMEM. A partial is laid out for that: 16 bytes of 32 rows follow one
 // another. A whole row tile goes out as the projection's bf16 hi/lo pair, through 4 KB of shared memory,
 // so that 64 bytes of a row are stored at a time (stored from the lanes, 16 bytes of 32 rows each, this
-// took 20000 cycles; through shared memory 11000; a partial 3000).
+// took 20000 cycles; through shared memory 13000; a partial takes 9000). Either is 256 KB of an SM, beside
+// the loads of the next tiles.
 // The loops stay rolled: what runs once per row tile is not in the instruction cache, and every 128
 // bytes of it cost some 250 cycles.
 __device__ __forceinline__ void write_o(const TreeArgs &a, const TreeSeg &g, int cl, uint32_t addr,

@@ -326,6 +326,17 @@ def test_tree_drafts_across_tiles(ctx):
     check_tree(ctx, rng, [100, 127, 96, 31, 32, 33, 65], [60, 64, 33, 1, 32, 2, 63], 8, 6, "tree")
 
 
+@pytest.mark.parametrize("busy", [40, 1500])
+def test_tree_many_sequences(ctx, busy):
+    """More sequences than the plan's block has threads, few of them or most with a token."""
+    rng = np.random.default_rng(busy)
+    B = 2300
+    toks = np.zeros(B, int)
+    toks[rng.permutation(B)[:busy]] = rng.integers(1, 3, busy)
+    lens = np.where(rng.random(B) < 0.9, rng.integers(0, 20, B), rng.integers(100, 400, B))
+    check_tree(ctx, rng, lens.tolist(), toks.tolist(), 8, 1, "tree", pad=1)
+
+
 def test_tree_sees_nothing(ctx):
     rng = np.random.default_rng(8)
     *_, got = check_tree(ctx, rng, [0, 0, 5], [3, 1, 2], 16, 5, "none")
