@@ -134,7 +134,6 @@ struct TreeArgs {
     const TreePlan *plan;
     const unsigned long long *mask;
     const __nv_bfloat16 *latent, *rope;  // the cache's rows
-    const __nv_bfloat16 *qlat; // [T][H][576]
     float *part;               // [2 TT_CLUSTERS][TT_PART]
     __nv_bfloat16 *olat2;      // [T][H][hi 512 | lo 512]
     float *rowsum;             // [T][H]
@@ -1074,7 +1073,7 @@ extern "C" int k3cuda_mla_tree_attend(k3cuda_ctx *ctx, void *out, int out_dtype,
     int *keep = (int *)(w + ws.keep);
     __nv_bfloat16 *qlat = (__nv_bfloat16 *)(w + ws.qlat);
     const TreeArgs a{paged_view(cache, batch), plan, tree_mask,
-                     (const __nv_bfloat16 *)cache->latent, (const __nv_bfloat16 *)cache->rope, qlat,
+                     (const __nv_bfloat16 *)cache->latent, (const __nv_bfloat16 *)cache->rope,
                      (float *)(w + ws.part), (__nv_bfloat16 *)(w + ws.olat2),
                      (float *)(w + ws.rowsum), H, scale_log2e, ctx->err_word};
     const uint64_t rows = (uint64_t)cache->n_pages * cache->page_size;
