@@ -819,8 +819,13 @@ __device__ __forceinline__ void value_output(const TreeArgs &a, TreeWalk walk, u
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.p_full[pb]);
             if ((long long)(t + 1) * TT_TILE <= sg.s.len) continue;
-            // rows past the cached ones: zero where nothing is written, and where a draft's element
-            // is not finite (a chunk without rows is left out of the products)
+            // Rows past the cached ones: zero where nothing is written, and where a draft's element
+            // is not finite (a chunk without rows is left out of the products). The last tile's
+            // products are waited for first. P may come before that tile's rows have, and the stages'
+            // barriers, of which a wait sees one bit, would show its phase as this tile's; and the MMA
+            // warp may still be about to look at `clean` for that tile, which the arrivals below
+            // would take a phase further.
+            if (g > 0 && !warp_spin(&bars.pv_done[before], ph, a.err, 0x556)) return;
             const int live = sg.s.len + sg.s.n - t * TT_TILE;
 #pragma unroll 1
             for (int c = 0; c < TT_VCH; c++) {

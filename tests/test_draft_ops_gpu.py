@@ -337,6 +337,23 @@ def test_tree_many_sequences(ctx, busy):
     check_tree(ctx, rng, lens.tolist(), toks.tolist(), 8, 1, "tree", pad=1)
 
 
+@pytest.mark.parametrize("lens,toks,page,H", [
+    ([100] * 160, [29] * 160, 8, 4),                   # a full tile of drafts, then one of one row
+    ([3 * 128 + 70, 2 * 128 - 1, 127] * 40, [64, 2, 33] * 40, 8, 2),
+    ([12000, 128, 5 * 128], [3, 1, 64], 16, 24)])
+def test_tree_tiles_past_the_cached_rows_wait_for_the_last(ctx, lens, toks, page, H):
+    """Tiles with drafts behind cached tiles and behind one another, the chunks of the second with
+    and without rows, row tile after row tile; the caches cold and warm, all with the same bits.
+    Unwritten rows hold NaN."""
+    rng = np.random.default_rng([len(lens), page, H])
+    p, x, words, got = check_tree(ctx, rng, lens, toks, page, H, "tree")
+    for k in range(12):
+        if k % 2:
+            ctx.flush_l2()
+        again = run_tree(ctx, p, x, words, H, 0.0722)
+        assert (again.view(np.uint32) == got.view(np.uint32)).all()
+
+
 def test_tree_sees_nothing(ctx):
     rng = np.random.default_rng(8)
     *_, got = check_tree(ctx, rng, [0, 0, 5], [3, 1, 2], 16, 5, "none")
