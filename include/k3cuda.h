@@ -320,7 +320,8 @@ int k3cuda_mla_tree_attend(k3cuda_ctx *ctx, void *out, int out_dtype, const void
  *   top_ids, top_logprobs  d [T][K]  the K likeliest tokens, likeliest first, equal logits in the
  *                           order of their numbers; places past the last token with a logit above
  *                           -inf hold -1 and -inf (K == 0: none)
- * in one pass over the logits, sums in fp32. A logit of -inf is a token that cannot come. A row
+ * in one pass over the logits, sums in fp32 (K passes more where over a thousand of the likeliest lie
+ * whole multiples of 1024 logits apart). A logit of -inf is a token that cannot come. A row
  * that holds a NaN or +inf, or nothing but -inf, has no distribution: NaN, ids -1.
  * K <= K3CUDA_MAX_TOP, V >= 1, any alignment of the rows to their element size. workspace d:
  * k3cuda_token_logprobs_workspace() bytes (which do for smaller T, V and K too), 256-byte aligned,

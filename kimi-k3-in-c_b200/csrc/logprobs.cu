@@ -9,12 +9,19 @@
 // clock and SM.
 //
 // The K likeliest tokens come out of the same pass. A thread writes the maximum of each group of
-// logits it reads (its cell) to shared memory. The K-th largest of some thread maxima is a bound
-// that at least K logits reach, so only cells that reach it are read again (from L2, a few dozen
-// of thousands): they are listed first and read all at once, since one after another, as each
-// thread meets its own, they took 13 us of a block. The handful of logits at or above the bound
-// are ranked by (logit, lower number). Where more cells or logits reach it than the buffers hold
-// (rows of equal logits), the block instead searches the row K times.
+// logits it reads (its cell) to shared memory. The K-th largest of the thread maxima is a bound that
+// at least K logits reach, so only cells that reach it are read again (from L2, a few dozen of
+// thousands): they are listed first and read all at once, since one after another, as each thread
+// meets its own, they took 13 us of a block. The handful of logits at or above the bound are ranked
+// by (logit, lower number). (The K-th largest of every warp's ceil(K / 8) best is a bound that is had
+// sooner, but where a few warps hold nothing but -inf there are too few of those, and all the others'
+// logits were ranked: 7 us.) The bound has the logit's upper 16 bits. Where more than LP_FEW
+// cells or logits reach those (fp32 logits far from zero, bf16 logits with equal ones at the top), it is found
+// again from the threads' best (logit, number) in 64 bits. Where even that leaves more than LP_CAND
+// (thousands of likely tokens in fewer than K threads: a period of 1024 or 4096 fp32 logits), the block
+// searches its segment K times. 512 x 163840 fp32, K = 20, by events: 77 us; 101 us with logits around
+// 1030 and 95 us with equal ones (2205 us both when those were searched K times); 3.3 ms where the
+// likely ones lie 1024 apart, K = 30.
 //
 // Rows are cut into segments of whole iterations when there are few of them: each block leaves
 // (m, s, t) and its K best, and a second kernel joins a row's segments.
@@ -34,6 +41,7 @@ namespace k3 {
 constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32;
 constexpr int LP_MAX_IT = 32;      // iterations of a segment (cells per thread)
 constexpr int LP_CAND = 1024;      // cells listed, candidates ranked at once
+constexpr int LP_FEW = 256;        // of either that are taken without looking for a closer bound
 constexpr int LP_MAX_SEG = 256;    // segments of a row
 constexpr int LP_MAX_V = 1 << 24;
 static_assert(K3CUDA_MAX_TOP * K3CUDA_MAX_TOP <= LP_CAND, "a join's candidates fit");
@@ -254,17 +262,13 @@ struct LpShared {
     u64 cand[LP_CAND], best[K3CUDA_MAX_TOP], wbest[LP_WARPS];
 };
 
-// The bound: at least K logits of the block are at or above it (LP_ORD_NINF + 1 where fewer than
-// K threads hold one above -inf). It is the K-th largest thread maximum to its upper 16 bits, found
-// bit by bit. (The K-th largest of every warp's ceil(K / 8) best is had sooner, but where a few warps
-// hold nothing but -inf there are too few of those, and all the others' logits were ranked: 7 us.)
-__device__ __forceinline__ unsigned block_bound(float m, int K) {
-    const unsigned mine = m == -INFINITY ? 0u : ord(m) >> 16;
-    unsigned at = 0;
+// The K-th largest of the threads' numbers (0 where fewer have one), bit by bit from `bit` on; `at`:
+// the bits above that.
+template <typename N> __device__ __forceinline__ N block_kth(N mine, int K, N at, N bit) {
 #pragma unroll 1
-    for (unsigned bit = 1u << 15; bit; bit >>= 1)
+    for (; bit; bit >>= 1)
         if (__syncthreads_count(mine >= (at | bit)) >= K) at |= bit;
-    return max(at << 16, LP_ORD_NINF + 1);
+    return at;
 }
 
 template <int U> __device__ __forceinline__ uint4 pick(const uint4 *r, int u) {
@@ -273,6 +277,25 @@ template <int U> __device__ __forceinline__ uint4 pick(const uint4 *r, int u) {
     for (int i = 1; i < U; i++)
         if (u == i) x = r[i];
     return x;
+}
+
+// This thread's best key: its largest logit m where that comes first (cells lie it, it + 1, .. one
+// after another). 0 without a logit above -inf.
+template <typename T, int U>
+__device__ __noinline__ u64 best_key(const Row<T> r, const float *cell, int v0, int v1, int its,
+                                     float m) {
+    constexpr int N = vec<T>::N;
+    if (m == -INFINITY) return 0;
+    int it = 0;
+    while (it < its - 1 && cell[it * LP_THREADS + threadIdx.x] != m) it++;
+    for (int u = 0; u < U; u++) {
+        const int v = v0 + (it * U + u) * LP_THREADS + threadIdx.x;
+        float x[N];
+        vec<T>::unpack(r.load(v, v1), x);
+        for (int i = 0; i < N; i++)
+            if (x[i] == m) return key_of(m, v * N - r.skew + i);
+    }
+    return 0;
 }
 
 // U: 16-byte vectors a thread reads per iteration
@@ -352,32 +375,46 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_k(const LpArgs a
     const float tm = st.m;
     const Stat all = block_join(st, sh.red);
     if (a.K) {
-        const unsigned bound = block_bound(tm, a.K);
-        if (tid == 0) sh.n = sh.cells = 0;
-        __syncthreads();
-        if (ord(tm) >= bound)
-            for (int it = 0; it < its; it++) {
-                if (ord(cell[it * LP_THREADS + tid]) < bound) continue;
-                const int p = atomicAdd(&sh.cells, 1);
-                if (p < LP_CAND) sh.list[p] = (unsigned short)(it * LP_THREADS + tid);
-            }
-        __syncthreads();
-        const int cells = sh.cells;
+        // The bound: at least K logits of the block are at or above it (any above -inf where fewer
+        // than K threads hold one). The K-th largest thread maximum to its upper 16 bits will do,
+        // unless too many logits share those. Then it is the K-th largest of the threads' best keys,
+        // which no two logits share.
+        unsigned top = block_kth<unsigned>(tm == -INFINITY ? 0u : ord(tm) >> 16, a.K, 0u, 1u << 15);
+        constexpr u64 least = (u64)(LP_ORD_NINF + 1) << 32;
+        u64 bound = max((u64)top << 48, least);
+        bool fits;
 #pragma unroll 1
-        for (int e = tid; e < min(cells, LP_CAND) * U * N; e += LP_THREADS) {
-            const int c = sh.list[e / (U * N)];
-            const int v = v0 + (c / LP_THREADS * U + e / N % U) * LP_THREADS + c % LP_THREADS;
-            const int i = v * N - r.skew + e % N;
-            if (v >= v1 || i < 0 || i >= r.V) continue;
-            const float x = io<T>::ld(r.x + i);
-            if (ord(x) < bound || !(x <= INFINITY)) continue;
-            const int p = atomicAdd(&sh.n, 1);
-            if (p < LP_CAND) sh.cand[p] = key_of(x, i);
+        for (bool exact = false;; exact = true) {
+            if (tid == 0) sh.n = sh.cells = 0;
+            __syncthreads();
+            if (key_of(tm, 0) >= bound)
+                for (int it = 0; it < its; it++) {
+                    const int i = (v0 + it * U * LP_THREADS + tid) * N - r.skew;  // the cell's first
+                    if (key_of(cell[it * LP_THREADS + tid], max(i, 0)) < bound) continue;
+                    const int p = atomicAdd(&sh.cells, 1);
+                    if (p < LP_CAND) sh.list[p] = (unsigned short)(it * LP_THREADS + tid);
+                }
+            __syncthreads();
+            const int cells = sh.cells, limit = exact ? LP_CAND : LP_FEW;
+#pragma unroll 1
+            for (int e = tid; cells <= limit && e < cells * U * N; e += LP_THREADS) {
+                const int c = sh.list[e / (U * N)];
+                const int v = v0 + (c / LP_THREADS * U + e / N % U) * LP_THREADS + c % LP_THREADS;
+                const int i = v * N - r.skew + e % N;
+                if (v >= v1 || i < 0 || i >= r.V) continue;
+                const float x = io<T>::ld(r.x + i);
+                if (!(x <= INFINITY) || key_of(x, i) < bound) continue;
+                const int p = atomicAdd(&sh.n, 1);
+                if (p < LP_CAND) sh.cand[p] = key_of(x, i);
+            }
+            __syncthreads();
+            fits = cells <= limit && sh.n <= limit;
+            if (fits || exact) break;
+            const u64 mine = best_key<T, U>(r, cell, v0, v1, its, tm);
+            bound = max(block_kth<u64>(mine, a.K, (u64)top << 48, 1ull << 47), least);
         }
-        __syncthreads();
-        const int n = sh.n;
-        if (cells <= LP_CAND && n <= LP_CAND) {
-            rank_keys(sh.cand, n, a.K, sh.best);
+        if (fits) {
+            rank_keys(sh.cand, sh.n, a.K, sh.best);
         } else {
             // the next best, K times
             u64 last = ~0ull;

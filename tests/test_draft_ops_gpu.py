@@ -631,6 +631,56 @@ def test_logprobs_few_tokens_allowed(ctx, bf16, T, V):
     check_lp(ctx, x, rng.integers(0, V, (T, 2)), 32 if T == 1 else 8, bf16)
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("T,V", [(2, 163840), (300, 50000)])
+def test_logprobs_likeliest_in_few_threads(ctx, bf16, T, V):
+    """Likely tokens that a few threads of a block read (they lie a fixed stride apart), all the
+    others far below; distinct and in classes of equal ones. Of 300 rows with 24 in 1024 more reach
+    the bound than are ranked at once."""
+    rng = np.random.default_rng([T, V])
+    for stride, some, K in ((4096, 40, 20), (1024, 24, 32), (8192, 64, 9), (2048, 16, 30)):
+        x = rng.standard_normal((T, V)).astype(np.float32)
+        x[:, np.arange(V) % stride < some] += 20
+        x[1::2] = np.round(x[1::2])
+        x = W.round_bf16(x) if bf16 else x
+        check_lp(ctx, x, rng.integers(0, V, (T, 1)), K, bf16)
+
+
+def lp_time(ctx, x, K):
+    """Shortest of several device times of a call, in ms, with cold caches."""
+    T, V = x.shape
+    d, n = ctx.upload(x), ctx.token_logprobs_workspace(T, V, K)
+    ws, lp = ctx.empty((max(n, 1),), np.uint8), ctx.empty((T, 1), np.float32)
+    dtok, ids = ctx.upload(np.zeros((T, 1), np.int32)), ctx.empty((T, K), np.int32)
+    tlp, best = ctx.empty((T, K), np.float32), 1e9
+    for k in range(6):
+        ctx.flush_l2()
+        ctx.record(0)
+        ctx.token_logprobs(d, T, V, dtok, 1, lp, ws, n, K=K, top_ids=ids, top_logprobs=tlp)
+        ctx.record(1)
+        ctx.sync()
+        best = min(best, ctx.elapsed_ms(0, 1)) if k > 1 else best
+    return best
+
+
+@pytest.mark.parametrize("T,V", [(600, 163840), (7, 163840), (64, 50257)])
+def test_logprobs_of_logits_with_a_large_offset(ctx, T, V):
+    """Distinct fp32 logits around -1030, 1030 and 2^20: what a row's softmax does not see does not
+    change its ids, and costs no further passes over the row; nor do equal logits."""
+    rng = np.random.default_rng([T, V])
+    z = rng.standard_normal((T, V)).astype(np.float32) * 2.5
+    for off in (-1030.0, 1030.0, 2.0 ** 20):
+        x = z + np.float32(off)
+        if T < 100:
+            check_lp(ctx, x, rng.integers(0, V, (T, 2)), 20, False)
+        else:
+            ids = run_lp(ctx, x, rng.integers(0, V, (T, 1)), 20, False)[2]
+            order = np.argsort(-x[::60], axis=1, kind="stable")[:, :20]
+            assert (ids[::60] == order).all()
+            if off < 2.0 ** 19:   # at 2^20 thousands of logits are equal
+                assert lp_time(ctx, x, 20) < 2 * lp_time(ctx, z, 20)
+
+
 def test_logprobs_nothing_to_do(ctx):
     run_lp(ctx, np.zeros((0, 50), np.float32), np.zeros((0, 1), np.int64), 3, False)
     run_lp(ctx, np.zeros((3, 50), np.float32), np.zeros((3, 0), np.int64), 0, False)
