@@ -262,8 +262,9 @@ typedef struct {
  *
  * page_table, ctx_lens and cu_tokens are DEVICE arrays, read when the kernels run: a captured
  * graph replays with what they hold then. The kernels check them. A sequence that breaks a rule
- * above is left out (its rows stay as they were) and a page number outside [0, n_pages) reads as
- * page 0 (and is not written); either way the next k3cuda_sync returns K3CUDA_ERR_ARG. */
+ * above is left out (its rows stay as they were), with an offset that falls, is negative or passes T
+ * all sequences behind it too, and a page number outside [0, n_pages) reads as page 0 (and is not
+ * written); each way the next k3cuda_sync returns K3CUDA_ERR_ARG. */
 typedef struct {
     const int *ctx_lens, *cu_tokens;
     int        B, T;

@@ -10,9 +10,9 @@
 //
 // Memory-bound: every value is read once and written once. One block per (token, 16 heads) and
 // one per token for the cache row, 128 threads with all loads of a thread issued before any
-// use; a token's 32 angles are formed once per block. Measured: 5058 tokens of 128 heads in fp32
-// 137 us, 5.6 TB/s of what has to be read and written (86 % of a copy's rate); 64 tokens of 16 heads
-// 7 us, of which the host's part of the call is most.
+// use; a token's 32 angles are formed once per block. Measured with cold caches: 5058 tokens of 128
+// heads in fp32 129 us, 5.9 TB/s of what has to be read and written (90 % of a copy's rate); 64 tokens of
+// 16 heads 7.2 us, of which the host's part of the call is most.
 #include "internal.cuh"
 #include "paged.cuh"
 
@@ -65,36 +65,62 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&p);
 }
 
-// The sequence of token t: the last b with cu[b] <= t, found 32 offsets at a time by a warp (one
-// memory latency for 32 sequences, two for 1024). The caller checks that t lies in it.
-__device__ __forceinline__ int token_seq(const int *cu, int B, int t, int lane) {
-    int lo = 0, n = B;  // the answer lies in [lo, lo + n)
-    while (n > 1) {
-        const int step = (n + 31) / 32, at = lo + lane * step;
-        const unsigned below = __ballot_sync(0xffffffffu, lane * step < n && cu[at] <= t);
-        const int k = below ? 31 - __clz(below) : 0;
-        n = min(step, n - k * step);
-        lo += k * step;
+// The sequence of token t, in every thread; -1 for a row of none, or of one that its offsets leave
+// out. The block looks all offsets over, since those before a sequence decide whether it counts. That
+// is one memory latency for 512 sequences, where a search takes two (338 tokens of 13 sequences, or 64
+// of 64: 0.1 us less; 5058 tokens of 3 prompts 128 us instead of 138; 1024 x 1 tokens of 16 heads 7.9
+// instead of 8.1). Many thousands pay for it (4096 x 1 34 us instead of 22, 16384 x 1 338 instead of 92).
+__device__ __forceinline__ int token_seq(const PagedView &v, int t, int2 *red) {
+    int hit = v.B, bad = v.B;  // the first sequence with row t, the first that is out of order
+    auto look = [&](int lo, int hi, int b) {
+        // as paged_in_order; negative offsets are large ones
+        if ((unsigned)lo > (unsigned)hi || (unsigned)hi > (unsigned)v.T) bad = min(bad, b);
+        else if (lo <= t && t < hi) hit = min(hit, b);
+    };
+    const int skew = (int)((uintptr_t)v.cu / 4 % 4);
+#pragma unroll 1
+    for (int b = 4 * threadIdx.x - skew; b < v.B; b += 4 * PA_THREADS) {
+        if (b >= 0 && b + 4 <= v.B) {
+            const int4 c = *reinterpret_cast<const int4 *>(v.cu + b);
+            const int end = v.cu[b + 4];
+            look(c.x, c.y, b);
+            look(c.y, c.z, b + 1);
+            look(c.z, c.w, b + 2);
+            look(c.w, end, b + 3);
+        } else {
+            for (int k = max(b, 0); k < min(b + 4, v.B); k++) look(v.cu[k], v.cu[k + 1], k);
+        }
     }
-    return lo;
+    hit = __reduce_min_sync(0xffffffffu, hit);
+    bad = __reduce_min_sync(0xffffffffu, bad);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_int2(hit, bad);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < PA_THREADS / 32; w++) {
+        hit = min(hit, red[w].x);
+        bad = min(bad, red[w].y);
+    }
+    return hit < bad ? hit : -1;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(PA_THREADS) mla_paged_append_k(const AppendArgs a) {
     __shared__ float2 turn[PA_DR / 2];  // (cos, sin) of the token's angles
     __shared__ double red[PA_THREADS / 32];
+    __shared__ int2 seq[PA_THREADS / 32];
     pdl_trigger();
     pdl_wait();
     const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
-    const int b = token_seq(a.v.cu, a.v.B, t, lane);
-    const PagedSeq s = paged_seq(a.v, b, a.v.T);
+    const int b = token_seq(a.v, t, seq);
     if (t == 0 && blockIdx.y == 0)  // one block looks every sequence over
         for (int c = tid; c < a.v.B; c += PA_THREADS) {
             const int code = paged_seq(a.v, c, a.v.T).code;
             if (code) atomicCAS(a.err + 1, 0u, (unsigned)code);
         }
+    if (b < 0) return;  // a padding row, or a sequence that was left out
+    const PagedSeq s = paged_seq(a.v, b, a.v.T);
     const int i = t - s.first;
-    if (i < 0 || i >= s.n) return;  // a padding row, or a sequence that was refused
+    if (i >= s.n) return;
     if (tid < PA_DR / 2) turn[tid] = make_float2(1.f, 0.f);
     if (a.inv_freq && tid < PA_DR / 2) {
         const int pos = a.positions ? a.positions[t] : s.len + i;

@@ -207,24 +207,37 @@ __global__ void __launch_bounds__(1024) mla_tree_plan(PagedView v, int H, TreePl
                                                       long long *cum, int *keep, int clusters,
                                                       unsigned *err) {
     __shared__ long long wsum[32], carry, all;
+    __shared__ int ordered;
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     for (int t = tid; t < v.T; t += 1024) keep[t] = 0;
-    if (tid == 0) carry = all = 0;
-    __syncthreads();
-    long long tiles = 0;
-    for (int b = tid; b < v.B; b += 1024) {
-        const PagedSeq s = paged_seq(v, b, K3CUDA_MAX_DRAFTS);
-        if (s.code) atomicCAS(err + 1, 0u, (unsigned)s.code);
-        tiles += ((long long)s.n * H + TT_M - 1) / TT_M * ((s.len + s.n + TT_TILE - 1) / TT_TILE);
+    if (tid == 0) {
+        carry = all = 0;
+        ordered = v.B;
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
-    if (lane == 0) atomicAdd((unsigned long long *)&all, (unsigned long long)tiles);
     __syncthreads();
+    long long tiles;
+    for (;;) {
+        tiles = 0;
+        for (int b = tid; b < v.B; b += 1024) {
+            const PagedSeq s = paged_seq(v, b, K3CUDA_MAX_DRAFTS);
+            if (s.code) atomicCAS(err + 1, 0u, (unsigned)s.code);
+            if (!paged_in_order(v, b)) atomicMin(&ordered, b);
+            tiles += ((long long)s.n * H + TT_M - 1) / TT_M * ((s.len + s.n + TT_TILE - 1) / TT_TILE);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+        if (lane == 0) atomicAdd((unsigned long long *)&all, (unsigned long long)tiles);
+        __syncthreads();
+        tiles = all;
+        if (ordered == v.B) break;
+        v.B = ordered;  // once more without the sequences from the first that is out of order
+        __syncthreads();
+        if (tid == 0) all = 0;
+        __syncthreads();
+    }
     // A cluster has one tile at least. With no more than that for each, a row tile's fixed work is
     // left out of account, or the clusters that its places fall to would have no tile.
-    tiles = all;
     const int G = (int)(tiles < clusters ? tiles : clusters);
     const int fixed = tiles > clusters ? TT_FIXED : 0;
     for (int b0 = 0; b0 < v.B; b0 += 1024) {

@@ -20,7 +20,8 @@ namespace k3 {
 // What a kernel found wrong in the device-side tables (word 1 of the error block).
 enum PagedError {
     PAGED_OK = 0,
-    PAGED_OFFSETS = 1,  // cu_tokens falls, is negative or ends past the token rows
+    PAGED_OFFSETS = 1,  // cu_tokens falls, is negative or ends past the token rows: this sequence
+                        // and all behind it are left out (paged_in_order)
     PAGED_LENGTH = 2,   // ctx_lens negative
     PAGED_DRAFTS = 3,   // more new tokens than the call takes per sequence
     PAGED_TABLE = 4,    // rows past the sequence's page table
@@ -36,6 +37,13 @@ struct PagedView {
     int B, T;
     int shift;          // log2 of page_size
 };
+
+// Whether sequence b's offsets are in order. The sequences that count are those before the first
+// whose offsets are not, so that no two of them have a row in common: a caller of paged_seq sees to
+// that.
+K3_HD bool paged_in_order(const PagedView &v, int b) {
+    return v.cu[b] >= 0 && v.cu[b] <= v.cu[b + 1] && v.cu[b + 1] <= v.T;
+}
 
 // Sequence b's new tokens: rows first .. first + n - 1 of the token arrays, behind `len` cached
 // rows. A sequence that breaks a rule has n = 0 and says why in `code`.

@@ -291,3 +291,57 @@ def test_struct_layout_matches_the_header(tmp_path):
                         str(src)], capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
     assert np.dtype(np.int32).itemsize == C.sizeof(C.c_int)
+
+
+ORDER_SRC = r"""
+#include <assert.h>
+#include <stdio.h>
+#include <random>
+#include <vector>
+#include "paged.cuh"
+using namespace k3;
+int main() {
+    std::mt19937 g(2);
+    auto rnd = [&](int lo, int hi) { return lo + (int)(g() % (unsigned)(hi - lo + 1)); };
+    int none = 0, all = 0;
+    for (int it = 0; it < 50000; it++) {
+        const int B = rnd(1, 7), T = rnd(0, 30);
+        std::vector<int> table(B, 0), lens(B, 0), cu(B + 1);
+        for (int i = 0; i <= B; i++) {
+            cu[i] = (i ? cu[i - 1] : rnd(0, 2)) + rnd(0, 6);
+            if (it % 2 && rnd(0, 4) == 0) cu[i] = rnd(0, 1) ? (int)g() : rnd(-3, 35);
+        }
+        const PagedView v{table.data(), 1, 64, 1, lens.data(), cu.data(), B, T, 6};
+        int n = 0;
+        while (n < B && paged_in_order(v, n)) n++;
+        // those that count: no code of the offsets, within the rows, each row in one at most
+        std::vector<int> owner(T, -1);
+        for (int b = 0; b < n; b++) {
+            const PagedSeq s = paged_seq(v, b, 1 << 20);
+            assert(s.code == PAGED_OK && s.n == cu[b + 1] - cu[b]);
+            for (int i = 0; i < s.n; i++) {
+                assert(owner.at(s.first + i) < 0);
+                owner[s.first + i] = b;
+            }
+        }
+        if (n < B) assert(paged_seq(v, n, 1 << 20).code == PAGED_OFFSETS);
+        none += n == 0;
+        all += n == B;
+    }
+    assert(none > 1000 && all > 1000);
+    puts("ok");
+    return 0;
+}
+"""
+
+
+@pytest.mark.skipif(not shutil.which("g++"), reason="no host C++ compiler")
+def test_sequences_in_order_share_no_row(tmp_path):
+    src, exe = tmp_path / "order.cpp", tmp_path / "order"
+    src.write_text(ORDER_SRC)
+    r = subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-D_GLIBCXX_ASSERTIONS",
+                        "-I" + os.path.join(ROOT, "kimi-k3-in-c_b200", "csrc"), str(src), "-o",
+                        str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout == "ok\n", r.stderr

@@ -66,6 +66,31 @@ class Paged:
         self.up()
 
 
+# offsets of three sequences in eight token rows, and how many of the sequences are in order
+OUT_OF_ORDER = [([0, 5, -4, 8], 1), ([0, 2, 1, 8], 1), ([0, 2, 5, 4], 2), ([0, 3, 9, 8], 1),
+                ([-1, 2, 5, 8], 0), ([0, 8, 3, 5], 1), ([2, 4, 4, 3], 2), ([0, 3, 2000000000, 8], 1),
+                ([0, 4, 6, 2000000000], 2), ([1, 0, 4, 8], 0)]
+
+
+def reports(ctx, text):
+    """The next sync reports a bad table."""
+    try:
+        ctx.sync()
+    except k3cuda.K3CudaError as e:
+        assert e.code == k3cuda.ERR_ARG and text in str(e), e
+    else:
+        pytest.fail("nothing reported")
+
+
+def out_of_order(ctx, rng, cu, good):
+    toks = [max(0, min(cu[b + 1] - cu[b], 8)) if b < good else 4 for b in range(3)]
+    p = Paged(ctx, rng, [20, 30, 10], toks, 16)
+    p.fill_drafts(rng)
+    p.cu, p.T = np.array(cu, np.int32), 8
+    p.up()
+    return p
+
+
 # ------------------------------------------------------------------------------- append
 def rotated(x, pos, inv_freq, style):
     """R_p x in 64 bits, and a bound of what fp32 rotation may be off: the angle's reduction
@@ -196,6 +221,42 @@ def test_append_reports_bad_tables(ctx):
             want = ct[a:a + n, :512].astype(np.float64)
             want /= np.sqrt((want ** 2).mean(-1, keepdims=True) + 1e-6)
             near(got[p.rows(b)[p.lens[b]:]], want)
+
+
+def test_append_offsets_at_any_alignment(ctx):
+    """Offsets that begin anywhere in a 16-byte vector, more of them than a block reads at once."""
+    rng = np.random.default_rng(17)
+    for shift in range(4):
+        for B in (1, 2, 5, 7, 530):
+            p = Paged(ctx, rng, rng.integers(0, 30, B), rng.integers(0, 4, B), 8, 1)
+            d = ctx.upload(np.concatenate([np.full(shift, -5), p.cu, [-5] * 4]).astype(np.int32))
+            p.batch.cu_tokens = d.ptr + 4 * shift
+            run_append(ctx, rng, p, 1, k3cuda.F32, k3cuda.ROPE_HALF)
+
+
+@pytest.mark.parametrize("cu,good", OUT_OF_ORDER)
+def test_append_offsets_out_of_order(ctx, cu, good):
+    """Sequences before the first offset that is out of order are appended; nothing else changes."""
+    rng = np.random.default_rng(14)
+    p = out_of_order(ctx, rng, cu, good)
+    ct, w = rng.standard_normal((8, 576)).astype(np.float32), np.ones(512, np.float32)
+    q = rng.standard_normal((8, 3, 192)).astype(np.float32)
+    dct, dw, dq = ctx.upload(ct), ctx.upload(w), ctx.upload(q)
+    qn, qr = (ctx.upload(np.full((8, 3, n), 0x1234, np.uint16)) for n in (128, 64))
+    ctx.mla_paged_append(p.cache, p.batch, dct, dw, 1e-6, q=dq, q_nope=qn, q_rope=qr, H=3)
+    reports(ctx, "cu_tokens")
+    lat, rope, gn, gr = p.d[0].numpy(), p.d[1].numpy(), qn.numpy(), qr.numpy()
+    rest, told = np.ones(len(lat), bool), np.zeros(8, bool)
+    for b in range(good):
+        t, row = slice(cu[b], cu[b + 1]), p.rows(b)[p.lens[b]:]
+        c = ct[t].astype(np.float64)
+        near(lat[row], c[:, :512] / np.sqrt((c[:, :512] ** 2).mean(-1, keepdims=True) + 1e-6))
+        near(rope[row], c[:, 512:])
+        near(gn[t], q[t, :, :128].astype(np.float64))
+        near(gr[t], q[t, :, 128:].astype(np.float64))
+        rest[row], told[t] = False, True
+    assert (lat[rest] == p.latent[rest]).all() and (rope[rest] == p.rope[rest]).all()
+    assert (gn[~told] == 0x1234).all() and (gr[~told] == 0x1234).all()
 
 
 # ------------------------------------------------------------------------- tree attention
@@ -479,6 +540,69 @@ def test_tree_reports_bad_tables(ctx):
         for b in good:
             t = slice(int(keep[2][b]), int(keep[2][b + 1]))
             assert (np.abs(got[t] - want[t]) <= lim[t]).all(), (what, b)
+
+
+@pytest.mark.parametrize("cu,good", OUT_OF_ORDER)
+def test_tree_offsets_out_of_order(ctx, cu, good):
+    """The sequences that the append takes, and no others."""
+    rng = np.random.default_rng(15)
+    p = out_of_order(ctx, rng, cu, good)
+    x = tree_inputs(ctx, rng, p, 4)
+    n = ctx.mla_tree_attend_workspace(3, 8, 4)
+    out, ws = ctx.empty((8, 4, 128), np.float32), ctx.empty((n,), np.uint8)
+    out.fill(0x4B)
+    ws.fill(0xFF)
+    dx = [ctx.upload(a) for a in x]
+    ctx.mla_tree_attend(out, dx[0], dx[1], p.cache, p.batch, dx[2], dx[3], 4, 0.0722, ws, n)
+    reports(ctx, "cu_tokens")
+    got, told = out.numpy(), np.zeros(8, bool)
+    for b in range(good):
+        told[cu[b]:cu[b + 1]] = True
+    words = np.zeros(8, np.uint64)
+    for b in range(good):
+        words[cu[b]:cu[b + 1]] = tree_words(rng, [p.toks[b]], "chain")
+    p.toks = [t if b < good else 0 for b, t in enumerate(p.toks)]
+    f = lambda a: W.bf16_to_f32(a).astype(np.float64)  # noqa: E731
+    want, lim = tree_oracle(p, words, *(f(a) for a in x), 0.0722)
+    assert (np.abs(got[told] - want[told]) <= lim[told]).all()
+    assert (got[~told].view(np.uint32) == 0x4B4B4B4B).all()
+
+
+def test_refused_sequences_stay_as_they_were(ctx):
+    """A sequence that another rule leaves out: its cache rows, queries and outputs."""
+    rng = np.random.default_rng(16)
+    for what, lens in (("length", [20, -1, 10]), ("table", [20, 1 << 20, 10]), ("drafts", [20, 30, 10])):
+        toks = [2, 65 if what == "drafts" else 3, 3]
+        p = Paged(ctx, rng, [20, 30, 10], toks, 16)
+        p.fill_drafts(rng)
+        p.lens = lens
+        p.up()
+        bad = slice(2, 2 + toks[1])
+        x = tree_inputs(ctx, rng, p, 4)
+        dx = [ctx.upload(a) for a in x]
+        n = ctx.mla_tree_attend_workspace(3, p.T, 4)
+        out, ws = ctx.empty((p.T, 4, 128), np.float32), ctx.empty((n,), np.uint8)
+        out.fill(0x4B)
+        ctx.mla_tree_attend(out, dx[0], dx[1], p.cache, p.batch, dx[2], dx[3], 4, 0.0722, ws, n)
+        reports(ctx, {"length": "negative", "table": "page table", "drafts": "more new"}[what])
+        got = out.numpy()
+        assert (got[bad].view(np.uint32) == 0x4B4B4B4B).all(), what
+        assert (np.delete(got, np.arange(p.T)[bad], 0).view(np.uint32) != 0x4B4B4B4B).all(), what
+        if what == "drafts":
+            continue   # the append takes any number of tokens
+        q = rng.standard_normal((p.T, 4, 192)).astype(np.float32)
+        dq, dct = ctx.upload(q), ctx.upload(rng.standard_normal((p.T, 576)).astype(np.float32))
+        dw = ctx.upload(np.ones(512, np.float32))
+        qn, qr = (ctx.upload(np.full((p.T, 4, m), 0x1234, np.uint16)) for m in (128, 64))
+        ctx.mla_paged_append(p.cache, p.batch, dct, dw, 1e-6, q=dq, q_nope=qn, q_rope=qr, H=4)
+        reports(ctx, {"length": "negative", "table": "page table", "drafts": "more new"}[what])
+        assert (qn.numpy()[bad] == 0x1234).all() and (qr.numpy()[bad] == 0x1234).all(), what
+        p.lens = [20, 30, 10]
+        rest = np.ones(len(p.latent), bool)
+        for b in (0, 2):
+            rest[p.rows(b)[p.lens[b]:]] = False
+        assert (p.d[0].numpy()[rest] == p.latent[rest]).all(), what
+        assert (p.d[1].numpy()[rest] == p.rope[rest]).all(), what
 
 
 # ------------------------------------------------------------------------ log probabilities
