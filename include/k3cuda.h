@@ -75,7 +75,8 @@ int  k3cuda_wait_selftest(k3cuda_ctx *ctx);
 /* The context's cudaStream_t, as an opaque pointer (for callers that order their own
  * work against this library's). */
 void *k3cuda_stream(k3cuda_ctx *ctx);
-/* Device memory (256-byte aligned). */
+/* Device memory (256-byte aligned). Memory that a graph does not use may be freed while it is
+ * captured. */
 int  k3cuda_malloc(k3cuda_ctx *ctx, void **dptr, size_t bytes);
 int  k3cuda_free(k3cuda_ctx *ctx, void *dptr);
 /* Page-locked host memory, for the host-buffer entry points' fast copies. */

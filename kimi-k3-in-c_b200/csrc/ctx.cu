@@ -78,6 +78,14 @@ static const char *paged_error_text(unsigned code) {
     return "a device-side table holds a bad entry";
 }
 
+// A free may come while this thread captures a graph (a garbage collector's, of buffers that the
+// graph does not use). It is no part of the graph, and in the thread's own mode would end the capture.
+struct OutsideCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 constexpr int PIN_SLOTS = 16;
 constexpr size_t PIN_SLOT = 512u << 10;
 
@@ -254,6 +262,7 @@ int k3cuda_malloc(k3cuda_ctx *ctx, void **dptr, size_t bytes) {
 int k3cuda_free(k3cuda_ctx *ctx, void *dptr) {
     int rc = enter(ctx);
     if (rc) return rc;
+    const OutsideCapture outside;
     if (dptr) K3_CUDA_TRY(cudaFree(dptr));
     return K3CUDA_OK;
 }
@@ -271,6 +280,7 @@ int k3cuda_host_alloc(k3cuda_ctx *ctx, void **hptr, size_t bytes) {
 int k3cuda_host_free(k3cuda_ctx *ctx, void *hptr) {
     int rc = enter(ctx);
     if (rc) return rc;
+    const OutsideCapture outside;
     if (hptr) K3_CUDA_TRY(cudaFreeHost(hptr));
     return K3CUDA_OK;
 }

@@ -945,6 +945,35 @@ def test_captured_step_replays_with_new_lengths(ctx):
         part[4].close()
 
 
+def test_buffers_freed_while_a_step_is_captured(ctx):
+    """Frees of device and page-locked memory, as a garbage collector may make them at any time,
+    do not end a capture."""
+    rng = np.random.default_rng(23)
+    H, V = 4, 501
+    p = Paged(ctx, rng, [60], [3], 16)
+    host, dev, bufs = step_data(ctx, rng, p, H, V)
+    dw = ctx.upload(tree_words(rng, p.toks, "chain"))
+    verify_step(ctx, p, dev, H, V, dw, bufs)
+    ctx.sync()
+    want = {n: bufs[n].numpy() for n in ("out", "lp", "ids")}
+    spare, pinned = [ctx.empty((1 << 20,), np.uint8) for _ in range(2)], ctx.host_alloc(4096)
+
+    def step():
+        spare[0].free()
+        verify_step(ctx, p, dev, H, V, dw, bufs)
+        ctx.host_free(pinned)
+        spare[1].free()
+
+    g = Graph(ctx, step)
+    for n in want:
+        bufs[n].zero()
+    g.replay()
+    ctx.sync()
+    for n, a in want.items():
+        assert np.array_equal(bufs[n].numpy(), a), n
+    g.close()
+
+
 def test_two_contexts_at_once(ctx):
     """Two contexts (streams) run steps on caches and workspaces of their own at the same time."""
     rng = np.random.default_rng(22)
