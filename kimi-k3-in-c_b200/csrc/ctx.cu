@@ -160,7 +160,7 @@ int k3cuda_init(int device, k3cuda_ctx **out) {
         if (e == cudaSuccess) e = cudaEventCreateWithFlags(&c->ev_k[i], cudaEventDisableTiming);
     }
     if (e == cudaSuccess) e = cudaMalloc((void **)&c->err_word, 256);
-    if (e == cudaSuccess) e = cudaMemset(c->err_word, 0, 256);
+    if (e == cudaSuccess) e = cudaMemsetAsync(c->err_word, 0, 256, c->stream);
     if (e == cudaSuccess) e = cudaEventCreateWithFlags(&c->ev_fence, cudaEventDisableTiming);
     c->comm_timeout_ms = 60000;
     if (e != cudaSuccess) {
@@ -221,7 +221,9 @@ int k3cuda_sync(k3cuda_ctx *ctx) {
     // met a bad entry in a device-side table leaves its in word 1
     unsigned code[2] = {0, 0};
     K3_CUDA_TRY(cudaMemcpy(code, ctx->err_word, sizeof code, cudaMemcpyDeviceToHost));
-    if (code[0] || code[1]) K3_CUDA_TRY(cudaMemset(ctx->err_word, 0, sizeof code));
+    // cleared in the stream's order: before the next kernel may write it
+    if (code[0] || code[1])
+        K3_CUDA_TRY(cudaMemsetAsync(ctx->err_word, 0, sizeof code, ctx->stream));
     if (code[0])
         return set_error(K3CUDA_ERR_TIMEOUT, "a device-side wait timed out (code 0x%x)", code[0]);
     if (code[1]) return set_error(K3CUDA_ERR_ARG, "%s", paged_error_text(code[1]));

@@ -259,6 +259,21 @@ def test_append_offsets_out_of_order(ctx, cu, good):
     assert (gn[~told] == 0x1234).all() and (gr[~told] == 0x1234).all()
 
 
+def test_each_bad_call_is_reported(ctx):
+    """A call that follows a report at once is reported too, a good one is not."""
+    rng = np.random.default_rng(18)
+    p = Paged(ctx, rng, [20], [2], 16)
+    bad = k3cuda.TokenBatch(ctx_lens=p.d[3].ptr, cu_tokens=p.d[4].ptr, B=1, T=1)   # the offsets pass T
+    dct = ctx.upload(rng.standard_normal((2, 576)).astype(np.float32))
+    dw = ctx.upload(np.ones(512, np.float32))
+    for k in range(200):
+        ctx.mla_paged_append(p.cache, bad, dct, dw, 1e-6)
+        reports(ctx, "cu_tokens")
+        if k % 2:
+            ctx.mla_paged_append(p.cache, p.batch, dct, dw, 1e-6)
+            ctx.sync()
+
+
 # ------------------------------------------------------------------------- tree attention
 def tree_words(rng, toks, kind):
     """Visibility words: `tree` random trees, `chain` every earlier draft, `none` nothing,
