@@ -103,6 +103,7 @@ constexpr int TT_OW = TT_DL / TT_GRP;      // dims of o of a warp in the value C
 constexpr int TT_WORKERS = 4 * TT_GRP;     // warps 2 ..
 constexpr int TT_THREADS = (3 + TT_WORKERS) * 32;
 constexpr int TT_CLUSTERS = 74;            // 148 SMs of a B200
+constexpr int TT_DRAIN = 1 << 17;          // clocks that a CTA stays after a wait that ran out
 constexpr int TT_FIXED = 4;                // a row tile's fixed work, in tiles
 // a partial, in floats: o [dims / 4][rows][4], m [rows], l [rows]
 constexpr int TT_PART_M = TT_DL * TT_M, TT_PART_L = TT_PART_M + TT_M, TT_PART = TT_PART_L + TT_M;
@@ -414,7 +415,7 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t u) {
 // the first; for the value CTA 32 rows x 512 dims. Chunk c of every tile is in stage c. In the score
 // CTA a row tile's queries come through the same stages before its first tile.
 template <bool kScore>
-__device__ __forceinline__ void tree_loads(const TreeMaps &maps, const TreeArgs &a, TreeWalk walk,
+__device__ __forceinline__ bool tree_loads(const TreeMaps &maps, const TreeArgs &a, TreeWalk walk,
                                            uint8_t *sm, TreeBars &bars) {
     constexpr int CH = kScore ? TT_KCH : TT_VCH, ROWS = kScore ? TT_TILE : TT_VROWS;
     constexpr int ST = kScore ? TT_KST : TT_VST;
@@ -502,10 +503,11 @@ __device__ __forceinline__ void tree_loads(const TreeMaps &maps, const TreeArgs 
         for (int c = 0; c < ST; c++)
             if ((loaded >> (2 * c)) & 3) mbar_wait_quiet(&bars.full[c], (loaded >> (2 * c)) & 2 ? 1 : 0);
     __syncwarp();
+    return ok;
 }
 
 // ---------------------------------------------------------------- score CTA
-__device__ __forceinline__ void score_mma(const TreeArgs &a, TreeWalk walk, uint8_t *sm,
+__device__ __forceinline__ bool score_mma(const TreeArgs &a, TreeWalk walk, uint8_t *sm,
                                           TreeBars &bars, uint32_t tbase) {
     constexpr uint32_t id = idesc_f16(128, TT_TILE, false, false);
     int g = 0, st = 0;                              // tiles; the next stage
@@ -518,10 +520,10 @@ __device__ __forceinline__ void score_mma(const TreeArgs &a, TreeWalk walk, uint
     while (walk.next(sg)) {
         // The queries into TMEM, 16 dims at a time, once the last row tile's scores are formed. (Taken
         // there by the softmax warps, a row tile's first scores came 5000 cycles later.)
-        if (g > 0 && !warp_spin(&bars.s_full[(g - 1) & 1], ((g - 1) >> 1) & 1, a.err, 0x511)) return;
+        if (g > 0 && !warp_spin(&bars.s_full[(g - 1) & 1], ((g - 1) >> 1) & 1, a.err, 0x511)) return false;
 #pragma unroll 1
         for (int c = 0; c < TT_KCH; c++) {
-            if (!data && !warp_spin(&bars.full[st], ph, a.err, 0x514)) return;
+            if (!data && !warp_spin(&bars.full[st], ph, a.err, 0x514)) return false;
             tc_fence_after();
             uint64_t q = sdesc_kmajor(smem_u32(sm + st * TT_KSTAGE));
             uint32_t d = tbase + TT_TM_Q + 64 * c;
@@ -538,8 +540,8 @@ __device__ __forceinline__ void score_mma(const TreeArgs &a, TreeWalk walk, uint
             const int sb = g & 1;
             const uint32_t d = tbase + TT_TM_S + sb * TT_TILE;
             uint32_t q = tbase + TT_TM_Q;
-            if (!room && !warp_spin(&bars.s_empty[sb], ((g >> 1) - 1) & 1, a.err, 0x512)) return;
-            if (!rope && !warp_spin(&bars.r_full, g & 1, a.err, 0x515)) return;
+            if (!room && !warp_spin(&bars.s_empty[sb], ((g >> 1) - 1) & 1, a.err, 0x512)) return false;
+            if (!rope && !warp_spin(&bars.r_full, g & 1, a.err, 0x515)) return false;
             tc_fence_after();
             {
                 const uint64_t qr = sdesc_kmajor(smem_u32(sm + TT_OFF_QR));
@@ -551,7 +553,7 @@ __device__ __forceinline__ void score_mma(const TreeArgs &a, TreeWalk walk, uint
             }
 #pragma unroll 1
             for (int c = 0; c < TT_KCH; c++) {
-                if (!data && !warp_spin(&bars.full[st], ph, a.err, 0x513)) return;
+                if (!data && !warp_spin(&bars.full[st], ph, a.err, 0x513)) return false;
                 tc_fence_after();
                 uint64_t b = sdesc(smem_u32(sm + st * TT_KSTAGE), 16, 2048);
                 const int used = st;
@@ -574,9 +576,10 @@ __device__ __forceinline__ void score_mma(const TreeArgs &a, TreeWalk walk, uint
             }
         }
     }
+    return true;
 }
 
-__device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, uint8_t *sm,
+__device__ __forceinline__ bool score_softmax(const TreeArgs &a, TreeWalk walk, uint8_t *sm,
                                               TreeBars &bars, uint32_t tbase, int cl) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int q4 = warp & 3, grp = (warp - 2) >> 2;  // lane quarter, group
@@ -610,7 +613,7 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
         for (int t = sg.t0; t < sg.t1; t++, g++) {
             const int sb = g & 1;
             float s[TT_CW];
-            if (!warp_spin(&bars.s_full[sb], (g >> 1) & 1, a.err, 0x523)) return;
+            if (!warp_spin(&bars.s_full[sb], (g >> 1) & 1, a.err, 0x523)) return false;
             tc_fence_after();
             const int p0 = t * TT_TILE + c0;
             if (p0 + TT_CW > sg.s.len || sign != 1.f) {  // past the cached rows: masked in TMEM
@@ -643,7 +646,7 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
 #pragma unroll
                 for (int j = 0; j < 4; j++) m4[j] = max3(m4[j], s[i + j], i + 4 < TT_CW ? s[i + 4 + j] : s[i + j]);
             float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale, o;
-            if (!share(mx, o)) return;
+            if (!share(mx, o)) return false;
             mx = fmaxf(mx, o);
             float f = 1.f;
             if (t == sg.t0) {
@@ -669,7 +672,7 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
             sum[0] = add2(sum[0], sum[1]);
             l += sum[0].x + sum[0].y;
             // P as the MMA will read it: 16-byte chunk ch of a row of 64 columns, swizzled
-            if (g >= 1 && !warp_spin<true>(&bars.p_ack, (g - 1) & 1, a.err, 0x524)) return;
+            if (g >= 1 && !warp_spin<true>(&bars.p_ack, (g - 1) & 1, a.err, 0x524)) return false;
 #pragma unroll
             for (int c = 0; c < TT_CW / 8; c++)
                 st16s(P + swz(row, c),
@@ -681,7 +684,7 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
         }
         // the row's sum
         float o;
-        if (!share(l, o)) return;
+        if (!share(l, o)) return false;
         const int lr = sg.mt * TT_M + row;
         if (grp == 0 && lr < sg.s.n * a.H) {
             const float lt = l + o;
@@ -693,10 +696,11 @@ __device__ __forceinline__ void score_softmax(const TreeArgs &a, TreeWalk walk, 
             }
         }
     }
+    return true;
 }
 
 // P to the peer as soon as it is written and the buffer there is free.
-__device__ __forceinline__ void score_send(const TreeArgs &a, TreeWalk walk, uint8_t *sm,
+__device__ __forceinline__ bool score_send(const TreeArgs &a, TreeWalk walk, uint8_t *sm,
                                            TreeBars &bars) {
     const uint32_t ps = smem_u32(sm + TT_OFF_PS), fs = smem_u32(sm + TT_OFF_FS);
     const uint32_t pd = map_peer(smem_u32(sm + TT_OFF_P), 1), fd = map_peer(smem_u32(sm + TT_OFF_F), 1);
@@ -707,8 +711,8 @@ __device__ __forceinline__ void score_send(const TreeArgs &a, TreeWalk walk, uin
     while (walk.next(sg)) {
         for (int t = sg.t0; t < sg.t1; t++, g++) {
             const int pb = g & 1;
-            if (!warp_spin(&bars.p_out, g & 1, a.err, 0x531)) return;
-            if (g >= 2 && !warp_spin(&bars.pv_done[pb], ((g >> 1) - 1) & 1, a.err, 0x532)) return;
+            if (!warp_spin(&bars.p_out, g & 1, a.err, 0x531)) return false;
+            if (g >= 2 && !warp_spin(&bars.pv_done[pb], ((g >> 1) - 1) & 1, a.err, 0x532)) return false;
             if (lead) {
                 bulk_send(pd + pb * TT_PBUF, ps, TT_PBUF, bar + 8 * pb);
                 bulk_send(fd + pb * TT_M * 4, fs, TT_M * 4, bar + 8 * pb);
@@ -717,13 +721,14 @@ __device__ __forceinline__ void score_send(const TreeArgs &a, TreeWalk walk, uin
         }
     }
     // the peer's last arrivals on this CTA's barriers
-    if (g > 0 && !warp_spin<true>(&bars.p_ack, (g - 1) & 1, a.err, 0x533)) return;
+    if (g > 0 && !warp_spin<true>(&bars.p_ack, (g - 1) & 1, a.err, 0x533)) return false;
     for (int k = g >= 2 ? g - 2 : 0; k < g; k++)
-        if (!warp_spin(&bars.pv_done[k & 1], (k >> 1) & 1, a.err, 0x534)) return;
+        if (!warp_spin(&bars.pv_done[k & 1], (k >> 1) & 1, a.err, 0x534)) return false;
+    return true;
 }
 
 // ---------------------------------------------------------------- value CTA
-__device__ __forceinline__ void value_mma(const TreeArgs &a, TreeWalk walk, uint8_t *sm,
+__device__ __forceinline__ bool value_mma(const TreeArgs &a, TreeWalk walk, uint8_t *sm,
                                           TreeBars &bars, uint32_t tbase) {
     constexpr uint32_t id = idesc_f16(128, 256, false, true);
     int g = 0, edges = 0;
@@ -734,12 +739,12 @@ __device__ __forceinline__ void value_mma(const TreeArgs &a, TreeWalk walk, uint
             const int pb = g & 1;
             const bool edge = (long long)(t + 1) * TT_TILE > sg.s.len;
             const int live = min(TT_TILE, sg.s.len + sg.s.n - t * TT_TILE);  // rows of the tile
-            if (!ready && !warp_spin(&bars.p_full[pb], (g >> 1) & 1, a.err, 0x541)) return;
+            if (!ready && !warp_spin(&bars.p_full[pb], (g >> 1) & 1, a.err, 0x541)) return false;
 #pragma unroll 1
             for (int c = 0; c < TT_VCH; c++) {
-                if (!data && !warp_spin(&bars.full[c], g & 1, a.err, 0x542)) return;
+                if (!data && !warp_spin(&bars.full[c], g & 1, a.err, 0x542)) return false;
                 if (edge && c * TT_VROWS < live && !warp_spin(&bars.clean[c], edges & 1, a.err, 0x543))
-                    return;
+                    return false;
                 tc_fence_after();
                 // 16 rows at a time: P's columns, the rows' 512 dims in two halves
                 const uint64_t kv = sdesc(smem_u32(sm + c * TT_VSTAGE), 1024, 8192);
@@ -766,6 +771,7 @@ __device__ __forceinline__ void value_mma(const TreeArgs &a, TreeWalk walk, uint
             edges += edge;
         }
     }
+    return true;
 }
 
 // Bring the rows of the tiles to come into L2 (both CTAs' loads find them there): the score CTA's
@@ -801,7 +807,7 @@ __device__ __forceinline__ void value_prefetch(const TreeArgs &a, TreeWalk walk,
     }
 }
 
-__device__ __forceinline__ void value_output(const TreeArgs &a, TreeWalk walk, uint8_t *sm,
+__device__ __forceinline__ bool value_output(const TreeArgs &a, TreeWalk walk, uint8_t *sm,
                                              TreeBars &bars, uint32_t tbase, int cl) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int q4 = warp & 3, grp = (warp - 2) >> 2;
@@ -816,15 +822,15 @@ __device__ __forceinline__ void value_output(const TreeArgs &a, TreeWalk walk, u
             const int pb = g & 1, before = (g - 1) & 1, ph = ((g - 1) >> 1) & 1;
             if (warp == 2 && lane == 0) mbar_expect_tx(&bars.p_in[pb], TT_PBUF + TT_M * 4);
             if (t == sg.t0 && g > 0) {  // the last row tile's o, before it is written over
-                if (!warp_spin(&bars.pv_done[before], ph, a.err, 0x551)) return;
+                if (!warp_spin(&bars.pv_done[before], ph, a.err, 0x551)) return false;
                 tc_fence_after();
                 write_o(a, old, cl, oaddr, stage, 32 * q4, TT_OW * grp, TT_OW);
             }
-            if (!warp_spin<true>(&bars.p_in[pb], (g >> 1) & 1, a.err, 0x552)) return;
+            if (!warp_spin<true>(&bars.p_in[pb], (g >> 1) & 1, a.err, 0x552)) return false;
             if (warp == 2 && lane == 0) mbar_arrive_cluster_relaxed(&bars.p_ack, 0);
             const float f = t == sg.t0 ? 1.f : fac[pb * TT_M];
             if (__any_sync(0xffffffffu, f != 1.f)) {
-                if (!warp_spin(&bars.pv_done[before], ph, a.err, 0x553)) return;
+                if (!warp_spin(&bars.pv_done[before], ph, a.err, 0x553)) return false;
                 tc_fence_after();
                 rescale_o(oaddr, TT_OW, f);
             }
@@ -838,12 +844,12 @@ __device__ __forceinline__ void value_output(const TreeArgs &a, TreeWalk walk, u
             // barriers, of which a wait sees one bit, would show its phase as this tile's; and the MMA
             // warp may still be about to look at `clean` for that tile, which the arrivals below
             // would take a phase further.
-            if (g > 0 && !warp_spin(&bars.pv_done[before], ph, a.err, 0x556)) return;
+            if (g > 0 && !warp_spin(&bars.pv_done[before], ph, a.err, 0x556)) return false;
             const int live = sg.s.len + sg.s.n - t * TT_TILE;
 #pragma unroll 1
             for (int c = 0; c < TT_VCH; c++) {
                 if (c * TT_VROWS < live) {
-                    if (!warp_spin(&bars.full[c], g & 1, a.err, 0x554)) return;
+                    if (!warp_spin(&bars.full[c], g & 1, a.err, 0x554)) return false;
                     const int d0 = max(0, sg.s.len - (t * TT_TILE + c * TT_VROWS));
                     const int d1 = live - c * TT_VROWS;
                     // a warp per row; a lane's 16 bytes of two 64-dim blocks
@@ -869,30 +875,35 @@ __device__ __forceinline__ void value_output(const TreeArgs &a, TreeWalk walk, u
         }
         old = sg;
     }
-    if (g > 0 && warp_spin(&bars.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, a.err, 0x555)) {
-        tc_fence_after();
-        write_o(a, old, cl, oaddr, stage, 32 * q4, TT_OW * grp, TT_OW);
-    }
+    if (g == 0) return true;
+    if (!warp_spin(&bars.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, a.err, 0x555)) return false;
+    tc_fence_after();
+    write_o(a, old, cl, oaddr, stage, 32 * q4, TT_OW * grp, TT_OW);
+    return true;
 }
 
 __device__ __forceinline__ void tree_roles(const TreeMaps &maps, const TreeArgs &a,
                                            const TreeWalk &walk, uint8_t *sm, TreeBars &bars,
                                            uint32_t tbase, int cl, bool score) {
     const int warp = threadIdx.x >> 5;
+    bool ok = true;
     if (warp == 0) {
-        if (score) tree_loads<true>(maps, a, walk, sm, bars);
-        else tree_loads<false>(maps, a, walk, sm, bars);
+        ok = score ? tree_loads<true>(maps, a, walk, sm, bars)
+                   : tree_loads<false>(maps, a, walk, sm, bars);
     } else if (warp == 1) {
-        if (score) score_mma(a, walk, sm, bars, tbase);
-        else value_mma(a, walk, sm, bars, tbase);
+        ok = score ? score_mma(a, walk, sm, bars, tbase) : value_mma(a, walk, sm, bars, tbase);
     } else if (warp == 2 + TT_WORKERS) {
-        if (score) score_send(a, walk, sm, bars);
+        if (score) ok = score_send(a, walk, sm, bars);
         else value_prefetch(a, walk, bars);
     } else if (score) {
-        score_softmax(a, walk, sm, bars, tbase, cl);
+        ok = score_softmax(a, walk, sm, bars, tbase, cl);
     } else {
-        value_output(a, walk, sm, bars, tbase, cl);
+        ok = value_output(a, walk, sm, bars, tbase, cl);
     }
+    // After a wait that ran out, the CTAs stay until what is still on its way has arrived: P to the
+    // peer, whose barrier alone would show it, and products in TMEM, which take some microseconds.
+    if (!ok)
+        for (const long long t0 = clock64(); clock64() - t0 < TT_DRAIN;) __nanosleep(1000);
 }
 
 __global__ void __launch_bounds__(TT_THREADS, 1) __cluster_dims__(2, 1, 1)
