@@ -151,7 +151,6 @@ struct TreeMaps {
 struct TreeSeg {
     int b, mt, t0, t1, tiles;
     PagedSeq s;
-    long long ustart;  // the row tile's first place
     __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == tiles; }
     // the partial's slot: the even one of a cluster for a row tile that began in an earlier cluster
     __device__ __forceinline__ int slot(int c) const { return 2 * c + (t0 == 0 ? 1 : 0); }
@@ -189,7 +188,6 @@ struct TreeWalk {
             g.b = b;
             g.mt = mt;
             g.s = s;
-            g.ustart = at;
             g.tiles = (int)(cost - fixed);
             g.t0 = (int)(c0 > first ? c0 - first : 0);
             g.t1 = (int)(c1 < first ? 0 : c1 - first < g.tiles ? c1 - first : g.tiles);
