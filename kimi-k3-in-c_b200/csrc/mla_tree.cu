@@ -779,11 +779,11 @@ __device__ __forceinline__ bool value_mma(const TreeArgs &a, TreeWalk walk, uint
 // to bring one tile to every cluster (without the wait the first scores came 15000 cycles later).
 __device__ __forceinline__ void value_prefetch(const TreeArgs &a, TreeWalk walk, TreeBars &bars) {
     const int lane = threadIdx.x & 31, box = min(a.v.page_size, TT_TILE);
-    const long long t0 = clock64();
     int g = 0;
     TreeSeg sg;
     while (walk.next(sg)) {
         for (int t = sg.t0; t < sg.t1; t++, g++) {
+            const long long t0 = clock64();
             while (g > *(volatile int *)&bars.tile + TT_AHEAD) {
                 __nanosleep(400);
                 if (*(volatile unsigned *)a.err || clock64() - t0 > wait_limit(a.err)) return;
