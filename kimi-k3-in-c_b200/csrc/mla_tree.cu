@@ -1026,7 +1026,8 @@ static int tree_shape(int B, int T, int H, int dn, int dr, int dl, int dv) {
     if (dn != TT_DN || dr != TT_DR || dl != TT_DL || dv != TT_DV)
         return set_error(K3CUDA_ERR_UNSUPPORTED,
                          "mla_tree_attend: dn=%d dr=%d dl=%d dv=%d not built", dn, dr, dl, dv);
-    K3_ARG_CHECK(T < (1 << 23), "mla_tree_attend: T=%d", T);
+    // the per-head products take 128 tokens to a row of their grid
+    K3_ARG_CHECK(T <= 65535 * 128, "mla_tree_attend: T=%d", T);
     return K3CUDA_OK;
 }
 

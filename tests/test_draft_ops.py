@@ -345,3 +345,16 @@ def test_sequences_in_order_share_no_row(tmp_path):
     assert r.returncode == 0, r.stderr
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0 and r.stdout == "ok\n", r.stderr
+
+
+def test_attend_takes_no_more_tokens_than_its_grids():
+    n = C.c_size_t()
+    for T, ok in ((65535 * 128, True), (65535 * 128 + 1, False), (1 << 23, False)):
+        q = lambda: k3cuda.lib().k3cuda_mla_tree_attend_workspace(  # noqa: E731
+            1, T, 1, 512, 128, C.byref(n))
+        if ok:
+            k3cuda.check(q())
+        else:
+            refused(q, k3cuda.ERR_ARG, f"T={T}")
+        refused(attend(cache(), batch(T=T), H=1), k3cuda.ERR_ARG,
+                "null context" if ok else f"T={T}")
