@@ -123,6 +123,7 @@ struct TreeStart {
 // the device-side plan, at the start of the workspace
 struct TreePlan {
     long long total;   // places on the line
+    int B;             // sequences that count
     int G;             // clusters that take part
     int fixed;         // places of a row tile's fixed work
     int cuts;
@@ -133,6 +134,7 @@ struct TreePlan {
 struct TreeArgs {
     PagedView v;
     const TreePlan *plan;
+    const long long *cum;      // the sequences' first places
     const unsigned long long *mask;
     const __nv_bfloat16 *latent, *rope;  // the cache's rows
     float *part;               // [2 TT_CLUSTERS][TT_PART]
@@ -156,6 +158,12 @@ struct TreeSeg {
     __device__ __forceinline__ int slot(int c) const { return 2 * c + (t0 == 0 ? 1 : 0); }
 };
 
+// The sequence that holds a place of the line (a step at a time, millions of empty ones took longer than
+// a wait may). Not expanded into the roles, which seldom need it.
+__device__ __noinline__ int tree_find(const long long *cum, int B, long long x) {
+    return last_at_most(cum, B, x);
+}
+
 struct TreeWalk {
     const TreeArgs &a;
     long long c0, c1, at;  // this cluster's places; the next row tile's first place
@@ -178,10 +186,14 @@ struct TreeWalk {
     }
     __device__ __forceinline__ bool next(TreeSeg &g) {
         while (at < c1) {
-            if (mt >= units) {  // the next sequence with tokens
+            if (mt >= units) {  // the next sequence with tokens, the one that holds place `at`
                 if (++b >= a.v.B) return false;
                 mt = 0;
                 seq();
+                if (units == 0) {
+                    b = tree_find(a.cum, a.plan->B, at);
+                    seq();
+                }
                 continue;
             }
             const long long first = at + fixed;  // place of tile 0
@@ -266,6 +278,7 @@ __global__ void __launch_bounds__(1024) mla_tree_plan(PagedView v, int H, TreePl
     if (tid == 0) {
         cum[v.B] = carry;
         plan->total = carry;
+        plan->B = v.B;
         plan->G = G;
         plan->fixed = fixed;
     }
@@ -1100,7 +1113,7 @@ extern "C" int k3cuda_mla_tree_attend(k3cuda_ctx *ctx, void *out, int out_dtype,
     long long *cum = (long long *)(w + ws.cum);
     int *keep = (int *)(w + ws.keep);
     __nv_bfloat16 *qlat = (__nv_bfloat16 *)(w + ws.qlat);
-    const TreeArgs a{paged_view(cache, batch), plan, tree_mask,
+    const TreeArgs a{paged_view(cache, batch), plan, cum, tree_mask,
                      (const __nv_bfloat16 *)cache->latent, (const __nv_bfloat16 *)cache->rope,
                      (float *)(w + ws.part), (__nv_bfloat16 *)(w + ws.olat2),
                      (float *)(w + ws.rowsum), H, scale_log2e, ctx->err_word};

@@ -430,6 +430,32 @@ def test_tree_tiles_past_the_cached_rows_wait_for_the_last(ctx, lens, toks, page
         assert (again.view(np.uint32) == got.view(np.uint32)).all()
 
 
+def test_tree_millions_of_empty_sequences(ctx):
+    """As many sequences as a call takes; few of them have tokens, and lie far apart."""
+    rng = np.random.default_rng(24)
+    B, k = (1 << 24) - 1, 160
+    p = Paged(ctx, rng, rng.integers(0, 250, k), rng.integers(1, 4, k), 256)   # a page each
+    p.fill_drafts(rng)
+    x = tree_inputs(ctx, rng, p, 2)
+    words = tree_words(rng, p.toks, "tree")
+    f = lambda a: W.bf16_to_f32(a).astype(np.float64)  # noqa: E731
+    want, lim = tree_oracle(p, words, *(f(a) for a in x), 0.0722)
+    at = np.arange(k) * (B // k) + rng.integers(0, B // k, k)
+    lens, n, table = np.full(B, 7, np.int32), np.zeros(B, np.int64), np.full(B, -3, np.int32)
+    lens[at], n[at], table[at] = p.lens, p.toks, p.table[:, 0]
+    cu = np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+    p.d[2:] = [ctx.upload(a) for a in (table, lens, cu)]
+    p.cache.max_pages, p.cache.page_table = 1, p.d[2].ptr
+    p.batch = k3cuda.TokenBatch(ctx_lens=p.d[3].ptr, cu_tokens=p.d[4].ptr, B=B, T=p.T)
+    m = ctx.mla_tree_attend_workspace(B, p.T, 2)
+    ws, out = ctx.empty((m,), np.uint8), ctx.empty((p.T, 2, 128), np.float32)
+    dx, dw = [ctx.upload(a) for a in x], ctx.upload(words)
+    ctx.mla_tree_attend(out, dx[0], dx[1], p.cache, p.batch, dx[2], dx[3], 2, 0.0722, ws, m,
+                        tree_mask=dw)
+    ctx.sync()
+    assert (np.abs(out.numpy() - want) <= lim).all()
+
+
 def test_tree_sees_nothing(ctx):
     rng = np.random.default_rng(8)
     *_, got = check_tree(ctx, rng, [0, 0, 5], [3, 1, 2], 16, 5, "none")
