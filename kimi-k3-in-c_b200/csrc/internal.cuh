@@ -141,17 +141,24 @@ int after_launch(k3cuda_ctx *ctx, const char *what);
 inline bool aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
 
 // ------------------------------------------------ programmatic dependent launch (PDL)
-// The kernels of a dependent chain (a layer's T <= 8 path) are launched with programmatic
-// stream serialization: the next kernel's CTAs are scheduled while the current one
+// The kernels of a dependent chain (a layer's T <= 8 path, the absorbed MLA decode and its per-head
+// products at any size, the operators over the paged cache, token log probabilities) are launched
+// with programmatic stream serialization: the next kernel's CTAs are scheduled while the current one
 // finishes, run their independent prologue (weight loads), and wait in pdl_wait() until the
 // previous kernel has completed and its writes are visible. A kernel calls pdl_wait() before
 // it reads anything an earlier kernel wrote and before its first global write; launched
 // without the attribute, pdl_wait() returns at once. pdl_trigger() lets the next kernel be
 // scheduled once every CTA of this one has issued it (its pdl_wait still waits for the end).
 // A kernel that does not call pdl_trigger lets its successor start only when it has finished,
-// as a plain launch would. The projections read weights before their pdl_wait, which is safe
-// because no kernel that calls pdl_trigger writes a weight matrix; a kernel that produces
-// weights (the MXFP4 expansion, the kv_b conversion) must keep not calling it.
+// as a plain launch would. Two rules go beyond one kernel:
+//   * The projections, mla_q_absorb_* and mla_project_* read weights before their pdl_wait, which is
+//     safe because no kernel that calls pdl_trigger writes a weight matrix; a kernel that produces
+//     weights (the MXFP4 expansion, the kv_b conversion) must keep not calling it.
+//   * mla_tree_plan reads the batch's tables and writes its plan before its pdl_wait, which comes at
+//     its end. That is safe because the kernel before it is always mla_q_absorb_tc or
+//     mla_q_absorb_small, and both trigger only after their own pdl_wait: when the plan starts, all
+//     that came before the absorption has completed. Both must keep that order, and nothing may come
+//     between them and the plan.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

@@ -136,7 +136,8 @@ mla_q_absorb_tc(const __grid_constant__ AbsorbMaps maps, unsigned *__restrict__ 
                 tma_load_3d(sB + (kb * 4 + nb) * 8192, &maps.b, &bar_ld, (4 * z + nb) * 64, kb * 64,
                             h);
     }
-    // The next kernel may start once every CTA is past the wait: what came before is done then.
+    // The next kernel may start once every CTA is past the wait: what came before is done then, and
+    // mla_tree_plan relies on it.
     // TMEM is taken after it too, so that no CTA holds any while an earlier kernel may want some.
     pdl_wait();
     pdl_trigger();
@@ -733,7 +734,7 @@ mla_q_absorb_small(const __nv_bfloat16 *__restrict__ q_nope,
             wv[j] = __ldg(reinterpret_cast<const uint4 *>(W + (size_t)(r0 + 16 * j) * MLA_DL));
     }
     pdl_wait();  // the weights above are never written by the chain; q_nope is
-    pdl_trigger();  // what came before is done when the next kernel starts
+    pdl_trigger();  // after the wait: mla_tree_plan relies on it (as in mla_q_absorb_tc)
     if (h >= H) {
         // a padding head of the MMA's M: its query row must score zero
         for (int e = tid; e < B * 128; e += 256)
