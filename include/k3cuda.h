@@ -303,9 +303,12 @@ int k3cuda_mla_paged_append(k3cuda_ctx *ctx, const k3cuda_paged_cache *cache,
  *   w_uk       d [H][dn][dl] bf16;  w_uv d [H][dv][dl] bf16
  * At most K3CUDA_MAX_DRAFTS new tokens per sequence. A token that sees nothing (no cached row,
  * no bit) gives zeros. What hidden or unwritten cache rows hold does not matter, infinities and
- * NaN included; a visible draft row that holds one gives NaN. Supported: dn == dv == 128,
+ * NaN included; a visible draft row that holds one gives NaN. As in k3cuda_mla_decode, the absorbed
+ * queries W_UK^T q_nope and the softmax weights are rounded to bf16 and summed in fp32: fp32 output keeps
+ * more digits of the result, it does not make it more accurate. Supported: dn == dv == 128,
  * dr == 64, dl == 512, H <= 128, scale finite. workspace d: k3cuda_mla_tree_attend_workspace()
- * bytes, 256-byte aligned, used by one call at a time. */
+ * bytes (39 MB of partial results, and 3.2 KB for each token and head), 256-byte aligned, used by
+ * one call at a time. */
 #define K3CUDA_MAX_DRAFTS 64
 int k3cuda_mla_tree_attend_workspace(int B, int T, int H, int dl, int dv, size_t *bytes);
 int k3cuda_mla_tree_attend(k3cuda_ctx *ctx, void *out, int out_dtype, const void *q_nope,

@@ -16,8 +16,8 @@
 // by (logit, lower number). (The K-th largest of every warp's ceil(K / 8) best is a bound that is had
 // sooner, but where a few warps hold nothing but -inf there are too few of those, and all the others'
 // logits were ranked: 7 us.) The bound has the logit's upper 16 bits. Where more than LP_FEW
-// cells or logits reach those (fp32 logits far from zero, bf16 logits with equal ones at the top), it is found
-// again from the threads' best (logit, number) in 64 bits. Where even that leaves more than LP_CAND
+// cells or logits reach those (fp32 logits far from zero, bf16 logits with equal ones at the top), it is
+// found again from the threads' best (logit, number) in 64 bits. Where even that leaves more than LP_CAND
 // (thousands of likely tokens in fewer than K threads: a period of 1024 or 4096 fp32 logits), the block
 // searches its segment K times. 512 x 163840 fp32, K = 20, by events: 77 us; 101 us with logits around
 // 1030 and 95 us with equal ones (2205 us both when those were searched K times); 3.3 ms where the
@@ -26,11 +26,12 @@
 // Rows are cut into segments of whole iterations when there are few of them: each block leaves
 // (m, s, t) and its K best, and a second kernel joins a row's segments.
 //
-// Measured: 512 rows of 163840 fp32 logits with the 20 likeliest 69 us (4.9 TB/s, 75 % of a copy's
-// rate; 59 us without the likeliest, whose work leaves a block's loads idle meanwhile); 2048 rows of
-// 163840 bf16 124 us (5.4 TB/s; the exponentials' unit is 68 % busy); one such row 10 us. Blocks that
-// begin their next segment's loads before they finish the last were slower (124 -> 149 us: segments
-// are dealt out unevenly then), and so was one segment instead of two for 512 rows (72 us).
+// Measured, the caches cold: 512 rows of 163840 fp32 logits with the 20 likeliest 69 us (4.9 TB/s, 74 %
+// of a copy's rate; 59 us without the likeliest, whose work leaves a block's loads idle meanwhile); 2048
+// rows of 163840 bf16 135 us (5.0 TB/s; back to back 124 us, the exponentials' unit 68 % busy); one such
+// row 9.2 us. Blocks that begin their next segment's loads before they finish the last were slower
+// (back to back 124 -> 149 us: segments are dealt out unevenly then), and so was one segment instead of
+// two for 512 rows (72 us).
 #include <algorithm>
 
 #include "internal.cuh"

@@ -33,7 +33,8 @@
 // Per SM:
 //   score   TMEM: query 256 columns, S 2 x 128;  shared: 5 stages of 32 KB (128 rows x 128 dims,
 //           K-major, a quarter of a tile), the tile's rope dims 16 KB, the query's 16 KB, P 32 KB on its
-//           way out (four stages and no reading ahead in the page table: 64 x 1 193 us, now 188)
+//           way out (four stages and no reading ahead in the page table: 64 x 1 193 us back to
+//           back, now 184)
 //   value   TMEM: o 512 columns;  shared: a tile in 4 stages of 32 KB (32 rows x 512 dims, MN-major),
 //           P 2 x 32 KB
 // Warps: 0 loads (a lane per page), 1 issues the MMAs, 2-9 are two groups of one warp per lane
@@ -49,14 +50,15 @@
 // The line is formed on the device from the batch's tables (mla_tree_plan), so that a captured
 // call follows them.
 //
-// Measured (the five launches of a call): 64 x 1 token of 128 heads over 8192 rows 188 us, of which this
-// kernel 160 (its floor is 97 us of HBM and 91 of MMAs); 48 x 13 tokens, 128 heads, 350 to 400 us as the
-// clock allows (300 in this kernel; 181 us of MMAs); one token after 509 rows 26 us. A tile takes about
-// 4250 cycles where its MMAs in the score CTA need 2650. What it waits for are the rows: 163 KB at 55 B a
-// clock, which share shared memory's 128 with the MMAs' reads of them and with P, and 91 cycles for each
-// of 10 TMA instructions (two pages of 64 rows; 18 instructions, a block of 64 dims each: 4600). 3870 of
-// the 4250 are the SM's own: so much it takes with 12 clusters at work instead of 74. A row tile's
-// start and end take some 14000 cycles.
+// Measured (the five launches of a call, the caches cold; in brackets calls back to back): 64 x 1 token of
+// 128 heads over 8192 rows 218 us (184), of which this kernel 153 (its floor is 97 us of HBM and 91 of
+// MMAs); 48 x up to 13 tokens, 128 heads, 393 to 406 us (350 to 383) as the clock allows (294 in this
+// kernel; 181 us of MMAs); one token after 509 rows 25 us (26). A tile takes about 4250 cycles where its
+// MMAs in the score CTA need 2650. 3870 of the 4250 are the SM's own: so much it takes with 12 clusters at
+// work instead of 74. What it waits for are the rows: 910 cycles for 10 TMA instructions (two pages of 64
+// rows, 91 cycles each; 18 instructions, a block of 64 dims each: 4600 cycles a tile), and 147 KB of rows
+// in the other 2960, 50 B a clock, beside the MMAs' reads of them and P in shared memory's 128. A row
+// tile's start and end take some 14000 cycles.
 //
 // Hidden rows: a masked score gives weight 0 whatever it is, and a zero weight times a row of
 // infinities must stay 0, so in tiles that reach past the cached rows the value CTA zeroes
