@@ -304,8 +304,8 @@ int k3cuda_mla_paged_append(k3cuda_ctx *ctx, const k3cuda_paged_cache *cache,
  * At most K3CUDA_MAX_DRAFTS new tokens per sequence. A token that sees nothing (no cached row,
  * no bit) gives zeros. What hidden or unwritten cache rows hold does not matter, infinities and
  * NaN included; a visible draft row that holds one gives NaN. As in k3cuda_mla_decode, the absorbed
- * queries W_UK^T q_nope and the softmax weights are rounded to bf16 and summed in fp32: fp32 output keeps
- * more digits of the result, it does not make it more accurate. Supported: dn == dv == 128,
+ * queries W_UK^T q_nope and the softmax weights are rounded to bf16 (all sums are fp32): fp32 output
+ * keeps more digits, it does not make the result more accurate than that. Supported: dn == dv == 128,
  * dr == 64, dl == 512, H <= 128, scale finite. workspace d: k3cuda_mla_tree_attend_workspace()
  * bytes (39 MB of partial results, and 3.2 KB for each token and head), 256-byte aligned, used by
  * one call at a time. */

@@ -67,9 +67,10 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 
 // The sequence of token t, in every thread; -1 for a row of none, or of one that its offsets leave
 // out. The block looks all offsets over, since those before a sequence decide whether it counts. That
-// is one memory latency for 512 sequences, where a search takes two (338 tokens of 13 sequences, or 64
-// of 64: 0.1 us less; 5058 tokens of 3 prompts 128 us instead of 138; 1024 x 1 tokens of 16 heads 7.9
-// instead of 8.1). Many thousands pay for it (4096 x 1 34 us instead of 22, 16384 x 1 338 instead of 92).
+// is one memory latency for 512 sequences, where a search takes two (16 heads, back to back: 64 x 1 tokens
+// 4.2 us instead of 4.3, 64 x 16 6.8 instead of 7.2, 1024 x 1 7.9 instead of 8.1; 5058 tokens of 3
+// prompts 129 instead of 138). Many thousands pay for it (4096 x 1 34 us instead of 22, 16384 x 1 338
+// instead of 92).
 __device__ __forceinline__ int token_seq(const PagedView &v, int t, int2 *red) {
     int hit = v.B, bad = v.B;  // the first sequence with row t, the first that is out of order
     auto look = [&](int lo, int hi, int b) {

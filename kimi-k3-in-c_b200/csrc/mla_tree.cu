@@ -533,7 +533,8 @@ __device__ __forceinline__ bool score_mma(const TreeArgs &a, TreeWalk walk, uint
     while (walk.next(sg)) {
         // The queries into TMEM, 16 dims at a time, once the last row tile's scores are formed. (Taken
         // there by the softmax warps, a row tile's first scores came 5000 cycles later.)
-        if (g > 0 && !warp_spin(&bars.s_full[(g - 1) & 1], ((g - 1) >> 1) & 1, a.err, 0x511)) return false;
+        if (g > 0 && !warp_spin(&bars.s_full[(g - 1) & 1], ((g - 1) >> 1) & 1, a.err, 0x511))
+            return false;
 #pragma unroll 1
         for (int c = 0; c < TT_KCH; c++) {
             if (!data && !warp_spin(&bars.full[st], ph, a.err, 0x514)) return false;
@@ -553,7 +554,8 @@ __device__ __forceinline__ bool score_mma(const TreeArgs &a, TreeWalk walk, uint
             const int sb = g & 1;
             const uint32_t d = tbase + TT_TM_S + sb * TT_TILE;
             uint32_t q = tbase + TT_TM_Q;
-            if (!room && !warp_spin(&bars.s_empty[sb], ((g >> 1) - 1) & 1, a.err, 0x512)) return false;
+            if (!room && !warp_spin(&bars.s_empty[sb], ((g >> 1) - 1) & 1, a.err, 0x512))
+                return false;
             if (!rope && !warp_spin(&bars.r_full, g & 1, a.err, 0x515)) return false;
             tc_fence_after();
             {
@@ -725,7 +727,8 @@ __device__ __forceinline__ bool score_send(const TreeArgs &a, TreeWalk walk, uin
         for (int t = sg.t0; t < sg.t1; t++, g++) {
             const int pb = g & 1;
             if (!warp_spin(&bars.p_out, g & 1, a.err, 0x531)) return false;
-            if (g >= 2 && !warp_spin(&bars.pv_done[pb], ((g >> 1) - 1) & 1, a.err, 0x532)) return false;
+            if (g >= 2 && !warp_spin(&bars.pv_done[pb], ((g >> 1) - 1) & 1, a.err, 0x532))
+                return false;
             if (lead) {
                 bulk_send(pd + pb * TT_PBUF, ps, TT_PBUF, bar + 8 * pb);
                 bulk_send(fd + pb * TT_M * 4, fs, TT_M * 4, bar + 8 * pb);
